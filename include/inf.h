@@ -280,6 +280,133 @@ Error_t inf_attn_decode_noalloc(const void* d_q, const void* d_kpool, const void
                                 u32 n_tokens, u32 n_heads, u32 n_kv_heads, u32 head_dim, u32 kv_block, u32 dtype,
                                 void* d_out, void* stream);
 
+/* ---- a paged KV cache of the caller's: write, attend, manage pages -------------------
+ * The entry points below work on a cache that the caller lays out.  They only enqueue work on
+ * `stream` (a cudaStream_t of the current device; all pointers are memory of that device): no
+ * allocation, no host synchronisation, so they can be captured into a CUDA graph and replayed with
+ * new contents of the same buffers.  What the host can see is checked before anything is
+ * launched (ErrorInvalidValue, ErrorInvalidDevPtr, ErrorUnsupported); what only the device can see
+ * (slots, positions, page ids, lengths) is checked by the kernels: they skip the offending part and
+ * store the first failure in the caller's status word (device i32, zero before the first call;
+ * NULL: not reported), which inf_check_status reads.  Scratch contents do not matter on entry; calls
+ * that can run at the same time need a scratch each. */
+typedef struct InfPagedKv {
+	void* kpool;        /* layer 0's K pool [n_pages][n_kv_heads][kv_block][head_dim], 16-byte aligned */
+	void* vpool;        /* layer 0's V pool, the same layout */
+	i32*  block_table;  /* [n_slots][pages_per_seq]: page of positions i * kv_block ..., -1: none */
+	i32*  page_refs;    /* [n_pages]: block-table entries that name the page (0: free); only inf_kv_free, _fork, _compact */
+	u64   layer_stride; /* bytes from one layer's pool to the next one's, K and V alike; a multiple of 16 */
+	u32   n_layers;
+	u32   n_slots;
+	u32   pages_per_seq;
+	u32   n_pages;
+	u32   n_kv_heads;
+	u32   head_dim;
+	u32   kv_block;     /* positions per page */
+	u32   dtype;        /* InfDtype */
+} InfPagedKv;
+/* Waits for `stream`, reads the status word, clears it and returns the failure it held (Success if
+ * none).  Not for a capturing stream. */
+Error_t inf_check_status(i32* d_status, void* stream);
+
+/* The projected rows of new tokens into the cache, one pass: per token and head, with x the head's
+ * head_dim values in fp32,
+ *   q and k:  y = x / sqrt(mean(x^2) + eps) * (gain_offset + gain)    (no gain array: y = x)
+ *             out_i = y_i cos_i - y_(i+h) sin_i,  out_(i+h) = y_(i+h) cos_i + y_i sin_i,  h = head_dim / 2, i < h,
+ *             cos and sin of the token's position
+ *   v:        copied
+ * rounded once.  Queries go to q_out, keys and values to row pos % kv_block of the page of pos in
+ * the slot's block table.  A row of qkv holds n_heads query heads, then n_kv_heads key heads, then
+ * as many value heads.  q_out may be qkv itself (same stride), otherwise they do not overlap.
+ * A token whose slot is negative is padding: nothing of it is read or written.  A slot or position
+ * outside the tables: reported (ErrorKvOutOfRange), the token skipped; a page outside the pool:
+ * reported, K and V not stored.  Two tokens at one position of one slot: which one the cache
+ * keeps is not determined.  head_dim * dtype size a multiple of 32 bytes, head_dim at most 512. */
+typedef struct InfQkNormRope {
+	const void* qkv;       /* [n_tokens] rows, 16-byte aligned */
+	void*       q_out;     /* [n_tokens] rows of n_heads * head_dim, 16-byte aligned */
+	u64         qkv_stride;   /* elements between rows; 0: (n_heads + 2 n_kv_heads) * head_dim */
+	u64         q_out_stride; /* elements between rows; 0: n_heads * head_dim */
+	const void* q_gain;    /* [head_dim] of the cache's dtype, 16-byte aligned; NULL: queries are not normalised */
+	const void* k_gain;    /* [head_dim]; NULL: keys are not normalised */
+	const f32*  rope_cos;  /* [n_pos][head_dim / 2], 16-byte aligned */
+	const f32*  rope_sin;
+	const i32*  tok_slot;  /* [n_tokens] */
+	const i32*  tok_pos;   /* [n_tokens] */
+	i32*        status;
+	f32         eps;
+	f32         gain_offset; /* 0, or 1 for (1 + gain) norms */
+	u32         n_pos;
+	u32         n_tokens;  /* 0: nothing to do */
+	u32         n_heads;
+	u32         layer;
+} InfQkNormRope;
+Error_t inf_qk_norm_rope(const InfPagedKv* kv, const InfQkNormRope* args, void* stream);
+
+/* Attention of the new tokens of a ragged batch over the paged cache, their own K and V already in
+ * it.  Sequence s has the rows q_start[s] .. q_start[s + 1] - 1 of q and out (none: it is
+ * skipped) and ctx_len[s] positions in its slot's pages, the new ones last: its row j is at
+ * position p = ctx_len[s] - rows + j and sees the positions k <= p with
+ *   window == 0  or  k > p - window  or  k < n_sink,
+ * out = sum_k softmax_k(scale * q . K_k) V_k, softmax statistics and sums in fp32, fp32 accumulation.
+ * bf16 caches with head_dim 64 or 128 and a kv_block of 16, 32, 64 or 128 run on the tensor cores (the
+ * weights are rounded to bf16 for the second product); others compute in fp32 throughout.
+ * A row that sees nothing (p < 0) gets zeros; rows before q_start[0] and from q_start[n_seqs] on are
+ * left as they were.  Pages that no row of a sequence sees may be missing (-1), and positions that no
+ * row sees may hold anything, NaN included.  Query heads h use KV head h / (n_heads / n_kv_heads).
+ * Rows outside q, more than max_new rows, a slot or context outside the tables: reported
+ * (ErrorInvalidValue / ErrorKvOutOfRange), the sequence skipped; a page outside the pool that a row
+ * sees: reported, the sequence's outputs unspecified.  n_seqs at most 4096. */
+typedef struct InfAttnChunk {
+	const void* q;         /* [n_tokens] rows of n_heads * head_dim, 16-byte aligned */
+	void*       out;       /* [n_tokens] rows of n_heads * head_dim, 16-byte aligned, not q */
+	u64         q_stride;  /* elements between rows, a multiple of 16 bytes; 0: n_heads * head_dim */
+	u64         out_stride;
+	const i32*  q_start;   /* [n_seqs + 1], not decreasing */
+	const i32*  ctx_len;   /* [n_seqs] */
+	const i32*  seq_slot;  /* [n_seqs]; NULL: sequence s is slot s */
+	void*       scratch;   /* inf_attn_chunk_scratch_bytes, 16-byte aligned */
+	u64         scratch_bytes;
+	i32*        status;
+	f32         scale;     /* > 0; 0: 1 / sqrt(head_dim) */
+	u32         n_seqs;    /* 0: nothing to do */
+	u32         n_tokens;  /* rows of q and out */
+	u32         max_new;   /* rows of a sequence at most (0: n_tokens); picks the kernels */
+	u32         n_heads;
+	u32         window;    /* 0: none */
+	u32         n_sink;
+	u32         layer;
+} InfAttnChunk;
+u64     inf_attn_chunk_scratch_bytes(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs);
+Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* stream);
+
+/* Pages.  All four are deterministic: indices are taken in order, free pages lowest id first. */
+/* Page d_dst[i] := page d_src[i] in every layer, K and V, for i < n.  A pair with an id outside the
+ * pool, a d_dst named by an earlier pair, or a d_dst that is some pair's d_src is reported
+ * (ErrorInvalidValue) and skipped.  Uses the pools only. */
+Error_t inf_kv_copy_pages(const InfPagedKv* kv, const i32* d_src, const i32* d_dst, u32 n, i32* d_status, void* stream);
+/* Entries d_first[i] .. d_last[i] - 1 of slot d_slot[i] are given up: each page they name loses one
+ * reference and the entry becomes -1 (d_first NULL: 0; d_last NULL: pages_per_seq).  An entry named
+ * twice is given up once.  Frees whole sequences, or the pages that left a sliding window.  A slot or
+ * range outside the table is reported (ErrorInvalidValue) and skipped, an entry outside the pool or a
+ * page without references too (the entry becomes -1). */
+Error_t inf_kv_free(const InfPagedKv* kv, const i32* d_slot, const i32* d_first, const i32* d_last, u32 n, i32* d_status,
+                    void* stream);
+/* Slot d_dst[i] becomes a copy of the first d_len[i] positions of slot d_src[i]: full pages are shared
+ * (one more reference each), a last partial page gets the lowest free page (in order of i) and its
+ * rows are copied in every layer.  Missing pages (-1) stay missing.  d_dst[i] must hold no pages, be
+ * named by no earlier fork and be no fork's source, and lengths must fit the table: else reported
+ * (ErrorInvalidValue) and skipped; skipped with ErrorArenaOutOfMemory when no page is free.
+ * d_scratch: inf_kv_pages_scratch_bytes, 16-byte aligned.  n at most n_slots. */
+Error_t inf_kv_fork(const InfPagedKv* kv, const i32* d_src, const i32* d_dst, const i32* d_len, u32 n, void* d_scratch,
+                    u64 scratch_bytes, i32* d_status, void* stream);
+/* The pages in use are brought to ids 0 .. *d_n_live - 1: with L of them, the i-th page in use at or
+ * above L moves, in every layer, to the i-th free id below L; references and block tables follow.
+ * d_map [n_pages] receives each old page's new id (-1: it was free).  n_pages at most 2^19. */
+Error_t inf_kv_compact(const InfPagedKv* kv, i32* d_map, i32* d_n_live, void* d_scratch, u64 scratch_bytes, i32* d_status,
+                       void* stream);
+u64     inf_kv_pages_scratch_bytes(const InfPagedKv* kv);
+
 /* ---- model ------------------------------------------------------------------------- */
 /* Built-in shapes: 1 tiny fp32 (d288), 2 TinyLlama-1.1B, 3 Llama-3-8B, 4 Llama-3-8B batch 64,
  * 5 Llama-3-8B 32k prefill, 6 the Gemma-4-E2B shape the reference's comments give

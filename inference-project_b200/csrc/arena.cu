@@ -36,6 +36,18 @@ bool is_device_ptr(const void* p)
 	return a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged;
 }
 
+bool is_local_device_ptr(const void* p)
+{
+	if (!p) return false;
+	cudaPointerAttributes a;
+	int dev = 0;
+	if (cudaPointerGetAttributes(&a, p) != cudaSuccess || cudaGetDevice(&dev) != cudaSuccess) {
+		cudaGetLastError();
+		return false;
+	}
+	return a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeDevice && a.device == dev);
+}
+
 } // namespace inf
 
 using inf::fail;

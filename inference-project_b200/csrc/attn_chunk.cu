@@ -1,0 +1,172 @@
+// inf_attn_chunk: attention of a ragged batch of new tokens over the paged cache.  Chooses the kernels
+// and their number of workers from what the host knows (types, head layout, row counts at most), lays
+// out the scratch, and enqueues them.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "k_attn_chunk.cuh"
+#include "launch.h"
+
+using namespace inf;
+
+namespace {
+
+u64 up256(u64 n) { return (n + 255) & ~255ull; }
+
+// One kernel's share of a call: the sequences with rows_min < rows <= rows_max rows per KV head.
+struct ChunkPass {
+	enum Kind { F32 } kind;
+	int rows_min, rows_max;
+	int workers, min_run;
+	int R, columns;      // row tile and layout of the partials
+	size_t smem;
+	u64 part_off, jobs_off;
+};
+
+struct ChunkPlan {
+	ChunkPass pass[2];
+	int n_pass;
+	u64 scratch;
+};
+
+// Items times key tiles at most.
+u64 units_max(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, u32 R, u32 KT)
+{
+	const u64 G = n_heads / kv->n_kv_heads;
+	const u64 tiles = (u64)n_tokens * G / R + std::min(n_seqs, n_tokens);
+	return tiles * kv->n_kv_heads * (((u64)kv->pages_per_seq * kv->kv_block + KT - 1) / KT + 1);
+}
+
+Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, ChunkPlan* P)
+{
+	const char* who = "inf_attn_chunk";
+	if (n_heads == 0 || n_heads > 65535 || n_heads % kv->n_kv_heads || n_seqs > (u32)kAcMaxSeqs ||
+	    (u64)n_tokens * (n_heads / kv->n_kv_heads) > (1u << 30))
+		return fail(ErrorInvalidValue, "%s: %u heads on %u KV heads, %u sequences, %u tokens", who, n_heads, kv->n_kv_heads, n_seqs,
+		            n_tokens);
+	const u64 es = kv->dtype == InfBF16 ? 2 : 4;
+	if (kv->head_dim > 512 || (kv->head_dim * es) % 16)
+		return fail(ErrorUnsupported, "%s: head_dim %u", who, kv->head_dim);
+	int sms = 148; // the scratch size is also asked for without a device
+	(void)sm_count(&sms);
+	P->n_pass = 0;
+	P->scratch = 0;
+	auto add = [&](ChunkPass p, u64 units) -> Error_t {
+		if (units > 0x7FFFFFFFull) return fail(ErrorUnsupported, "%s: %u tokens of %u positions at most", who, n_tokens, kv->pages_per_seq * kv->kv_block);
+		p.workers = (int)std::max<u64>(1, std::min<u64>(p.workers, (units + p.min_run - 1) / p.min_run));
+		p.part_off = P->scratch;
+		P->scratch += up256((u64)2 * p.workers * ac_part_floats(p.R, (int)kv->head_dim) * sizeof(float));
+		p.jobs_off = P->scratch;
+		P->scratch += up256((u64)p.workers * kAcJobInts * sizeof(int));
+		P->pass[P->n_pass++] = p;
+		return Success;
+	};
+	ChunkPass f = {};
+	f.kind = ChunkPass::F32;
+	f.rows_max = 0x7FFFFFFF;
+	f.R = kAfR;
+	f.min_run = 2;
+	f.smem = attn_chunk_f32_smem((int)kv->head_dim, (int)n_seqs);
+	f.workers = sms * (int)std::max<u64>(1, std::min<u64>(8, (200u << 10) / f.smem));
+	return add(f, units_max(kv, n_heads, n_tokens, n_seqs, kAfR, kAfKT));
+}
+
+template <typename T>
+Error_t launch_f32(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
+{
+	void (*k)(const AttnChunkArgs) = a.hd <= 128 ? k_attn_chunk_f32<T, 1> : a.hd <= 256 ? k_attn_chunk_f32<T, 2> : k_attn_chunk_f32<T, 4>;
+	INF_TRY(allow_smem(k, attn_chunk_f32_smem(a.hd <= 128 ? 128 : a.hd <= 256 ? 256 : 512, kAcMaxSeqs)));
+	return launch_pdl(k, dim3((unsigned)p.workers), dim3(kAfThreads), p.smem, st, a);
+}
+
+} // namespace
+
+extern "C" {
+
+u64 inf_attn_chunk_scratch_bytes(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs)
+{
+	ChunkPlan P;
+	if (!kv || kv->n_kv_heads == 0 || kv->kv_block == 0 || chunk_plan(kv, n_heads, n_tokens, n_seqs, &P) != Success) return 0;
+	return P.scratch;
+}
+
+Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* stream)
+{
+	const char* who = "inf_attn_chunk";
+	if (!args) return fail(ErrorInvalidValue, "%s: no arguments", who);
+	const InfAttnChunk& A = *args;
+	INF_TRY(check_paged_kv(who, kv, A.layer, true));
+	ChunkPlan P;
+	INF_TRY(chunk_plan(kv, A.n_heads, A.n_tokens, A.n_seqs, &P));
+	const u64 es = kv->dtype == InfBF16 ? 2 : 4, row = (u64)A.n_heads * kv->head_dim;
+	const u64 qs = A.q_stride ? A.q_stride : row, os = A.out_stride ? A.out_stride : row;
+	if (qs < row || os < row || qs > (1ull << 40) || os > (1ull << 40) || (qs * es) % 16 || (os * es) % 16)
+		return fail(ErrorInvalidValue, "%s: row strides", who);
+	if (!(A.scale >= 0.0f) || !std::isfinite(A.scale)) return fail(ErrorInvalidValue, "%s: scale %g", who, A.scale);
+	if (A.n_seqs == 0 || A.n_tokens == 0) return Success;
+	if (A.q == A.out) return fail(ErrorInvalidValue, "%s: out is q", who);
+	if (A.scratch_bytes < P.scratch) return fail(ErrorInvalidValue, "%s: scratch needs %llu bytes", who, (unsigned long long)P.scratch);
+	INF_TRY(check_paged_kv_pointers(who, kv, true, false));
+	INF_TRY(check_dev_arg(who, "q", A.q, 16));
+	INF_TRY(check_dev_arg(who, "out", A.out, 16));
+	INF_TRY(check_dev_arg(who, "q_start", A.q_start, 4));
+	INF_TRY(check_dev_arg(who, "ctx_len", A.ctx_len, 4));
+	if (A.seq_slot) INF_TRY(check_dev_arg(who, "seq_slot", A.seq_slot, 4));
+	INF_TRY(check_dev_arg(who, "scratch", A.scratch, 16));
+	INF_TRY(check_status_arg(who, A.status));
+	AttnChunkArgs a;
+	memset(&a, 0, sizeof a);
+	a.q = A.q;
+	a.out = A.out;
+	a.q_stride = qs;
+	a.out_stride = os;
+	const u64 off = kv->n_layers > 1 ? (u64)A.layer * kv->layer_stride : 0;
+	a.kpool = (const uint8_t*)kv->kpool + off;
+	a.vpool = (const uint8_t*)kv->vpool + off;
+	a.table = kv->block_table;
+	a.q_start = A.q_start;
+	a.ctx_len = A.ctx_len;
+	a.seq_slot = A.seq_slot;
+	a.n_seqs = (int)A.n_seqs;
+	a.n_tokens = (int)A.n_tokens;
+	a.max_new = (int)(A.max_new ? std::min(A.max_new, A.n_tokens) : A.n_tokens);
+	a.H = (int)A.n_heads;
+	a.KV = (int)kv->n_kv_heads;
+	a.G = a.H / a.KV;
+	a.hd = (int)kv->head_dim;
+	a.blk = (int)kv->kv_block;
+	a.n_slots = (int)kv->n_slots;
+	a.pages_per_seq = (int)kv->pages_per_seq;
+	a.n_pages = (int)kv->n_pages;
+	// a window that no context outgrows hides nothing
+	a.window = A.window >= kv->pages_per_seq * kv->kv_block ? 0 : (int)A.window;
+	a.n_sink = (int)std::min(A.n_sink, 1u << 30);
+	a.scale = A.scale > 0.0f ? A.scale : (float)(1.0 / std::sqrt((double)kv->head_dim));
+	a.status = A.status;
+	const cudaStream_t st = (cudaStream_t)stream;
+	auto pass_args = [&](const ChunkPass& p) {
+		AttnChunkArgs b = a;
+		b.rows_min = p.rows_min;
+		b.rows_max = p.rows_max;
+		b.workers = p.workers;
+		b.min_run = p.min_run;
+		b.part = (float*)((uint8_t*)A.scratch + p.part_off);
+		b.jobs = (int*)((uint8_t*)A.scratch + p.jobs_off);
+		return b;
+	};
+	for (int i = 0; i < P.n_pass; ++i) {
+		const AttnChunkArgs b = pass_args(P.pass[i]);
+		INF_TRY(kv->dtype == InfBF16 ? launch_f32<bf16>(b, P.pass[i], st) : launch_f32<float>(b, P.pass[i], st));
+	}
+	for (int i = 0; i < P.n_pass; ++i) {
+		const ChunkPass& p = P.pass[i];
+		const AttnChunkArgs b = pass_args(p);
+		const dim3 grid((unsigned)p.workers, (unsigned)((p.R + 31) / 32));
+		INF_TRY(launch_pdl(kv->dtype == InfBF16 ? k_attn_chunk_combine<bf16> : k_attn_chunk_combine<float>, grid, dim3(256), 0, st, b,
+		                   p.R, p.columns));
+	}
+	return Success;
+}
+
+} // extern "C"

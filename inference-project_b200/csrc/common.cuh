@@ -24,6 +24,8 @@ enum DevErr : int {
 	kDevTimeout = 1,
 	kDevTokenRange = 2,
 	kDevKvRange = 3,
+	kDevNoPages = 4,  // the KV pool has no free page left
+	kDevBadIndex = 5, // an index or length out of range, named twice or not free
 };
 
 // A bounded wait gives up after this long; the kernel then records kDevTimeout and

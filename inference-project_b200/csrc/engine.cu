@@ -9,6 +9,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <functional>
@@ -167,11 +168,7 @@ struct InfEngine {
 	float prof_ms[InfKNumKinds] = {};
 };
 
-namespace {
-
-enum CtlWord { kCtlId = 0, kCtlPos = 1, kCtlSlot = 2, kCtlStep = 3, kCtlErr = 4, kCtlEpoch = 5, kCtlWords = 8 };
-
-std::mutex g_attr_mutex;
+namespace inf {
 
 Error_t map_dev_err(int v)
 {
@@ -180,9 +177,51 @@ Error_t map_dev_err(int v)
 	case kDevTimeout: return fail(ErrorTimeout, "a bounded device wait expired");
 	case kDevTokenRange: return fail(ErrorTokenOutOfRange, "token id >= vocab_size");
 	case kDevKvRange: return fail(ErrorKvOutOfRange, "KV position or page outside the cache");
+	case kDevNoPages: return fail(ErrorArenaOutOfMemory, "the KV pool has no free page left");
+	case kDevBadIndex: return fail(ErrorInvalidValue, "an index or length on the device is out of range, named twice or not free");
 	default: return fail(ErrorGeneric, "device error word %d", v);
 	}
 }
+
+// The driver's tensor-map encoder, looked up once.
+static Error_t tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000* out)
+{
+	static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> encode{nullptr};
+	PFN_cuTensorMapEncodeTiled_v12000 f = encode.load(std::memory_order_acquire);
+	if (!f) {
+		cudaDriverEntryPointQueryResult q;
+		void* fn = nullptr;
+		INF_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+		if (q != cudaDriverEntryPointSuccess || !fn) return fail(ErrorCuda, "cuTensorMapEncodeTiled unavailable");
+		f = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+		encode.store(f, std::memory_order_release);
+	}
+	*out = f;
+	return Success;
+}
+
+Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages, u32 box_rows)
+{
+	PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+	INF_TRY(tensor_map_encoder(&encode));
+	const cuuint64_t dims[4] = {hd, blk, kv, pages};
+	const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)blk * hd * 2, (cuuint64_t)kv * blk * hd * 2};
+	const cuuint32_t box[4] = {64, box_rows ? box_rows : blk, 1, box_pages};
+	const cuuint32_t estr[4] = {1, 1, 1, 1};
+	const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+	                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+	                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+	if (r != CUDA_SUCCESS) return fail(ErrorCuda, "cuTensorMapEncodeTiled (K/V pool) failed (%d)", (int)r);
+	return Success;
+}
+
+} // namespace inf
+
+namespace {
+
+enum CtlWord { kCtlId = 0, kCtlPos = 1, kCtlSlot = 2, kCtlStep = 3, kCtlErr = 4, kCtlEpoch = 5, kCtlWords = 8 };
+
+std::mutex g_attr_mutex;
 
 Error_t check_dev_err(InfEngine* e)
 {
@@ -386,7 +425,6 @@ Error_t attn_cl_choose(InfEngine* e, int G, int hd)
 	                    &e->attn_cl_pages);
 }
 
-Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages);
 
 // launch with a cluster of cluster_x CTAs along x and the programmatic-dependency edge
 template <typename... KArgs, typename... Args>
@@ -783,42 +821,18 @@ Error_t enqueue_step(InfEngine* e)
 
 // --------------------------------------------------------------------------- prefill
 constexpr u64 kGemmPartBytes = 16ull << 20; // split-K scratch of the tensor-core GEMM
-PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-
 Error_t tensor_map_2d(CUtensorMap* m, const void* base, u64 rows, u64 cols, u32 box_rows)
 {
-	if (!g_encode) {
-		cudaDriverEntryPointQueryResult q;
-		void* fn = nullptr;
-		INF_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
-		if (q != cudaDriverEntryPointSuccess || !fn) return fail(ErrorCuda, "cuTensorMapEncodeTiled unavailable");
-		g_encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
-	}
+	PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+	INF_TRY(tensor_map_encoder(&encode));
 	const cuuint64_t dims[2] = {cols, rows};
 	const cuuint64_t strides[1] = {cols * 2};
 	const cuuint32_t box[2] = {(cuuint32_t)kTcBK, box_rows};
 	const cuuint32_t estr[2] = {1, 1};
-	const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-	                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-	                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+	const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+	                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+	                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 	if (r != CUDA_SUCCESS) return fail(ErrorCuda, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-	return Success;
-}
-
-// A layer's paged K or V pool [pages][KV][blk][hd] as a 4-D tensor (hd, row, head, page) with
-// boxes of 64 head dims x blk rows x 1 head x box_pages pages, SWIZZLE_128B.
-Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages)
-{
-	CUtensorMap dummy;
-	INF_TRY(tensor_map_2d(&dummy, base, 8, 64, 8)); // resolves the driver entry point
-	const cuuint64_t dims[4] = {hd, blk, kv, pages};
-	const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)blk * hd * 2, (cuuint64_t)kv * blk * hd * 2};
-	const cuuint32_t box[4] = {64, blk, 1, box_pages};
-	const cuuint32_t estr[4] = {1, 1, 1, 1};
-	const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-	                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-	                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-	if (r != CUDA_SUCCESS) return fail(ErrorCuda, "cuTensorMapEncodeTiled (K/V pool) failed (%d)", (int)r);
 	return Success;
 }
 

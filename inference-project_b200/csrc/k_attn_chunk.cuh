@@ -1,0 +1,509 @@
+// Attention of a ragged batch of new tokens over the paged cache: what its kernels share (the work
+// items, their division among workers, the joining of split rows) and the fp32 kernel that serves
+// every type and head size.
+//
+// An item is (sequence, KV head, row tile): the rows of a sequence and KV head are its new tokens times
+// the G query heads of the group, row r = token * G + head, R of them to a tile, so K and V are read
+// once per tile for the whole group.  The keys an item sees come in key tiles of KT positions: those of
+// the sinks, then those from the window's start to the last row's position; their number is the item's
+// cost.  All costs laid end to end (sequence, head, tile) are cut into equal runs, one per worker: a
+// worker may begin inside one item and end inside another, and every worker has the same number of key
+// tiles whatever the lengths are.  Where a cut falls inside an item each worker stores its share
+// (O, max, sum), and k_attn_chunk_combine joins them in the workers' order, so a result does not depend
+// on which worker finishes first.  Every warp finds its run from the lengths on the device: the host
+// needs none of them, and a captured launch follows new lengths.
+#pragma once
+
+#include "common.cuh"
+
+namespace inf {
+
+constexpr int kAcMaxSeqs = 4096;
+
+struct AttnChunkArgs {
+	const void* q;
+	void* out;
+	uint64_t q_stride, out_stride; // elements
+	const void* kpool;             // this layer's pages
+	const void* vpool;
+	const int* table;
+	const int* q_start;
+	const int* ctx_len;
+	const int* seq_slot;           // null: sequence s is slot s
+	int n_seqs, n_tokens, max_new;
+	int H, KV, G, hd, blk;
+	int n_slots, pages_per_seq, n_pages;
+	int window, n_sink;            // window 0: none
+	float scale;
+	int* status;
+	// division of the work: sequences with more than rows_min and at most rows_max rows per KV head
+	// belong to this launch
+	int rows_min, rows_max;
+	int workers;
+	int min_run;                   // key tiles of a worker at least
+	float* part;                   // [2 * workers][R][hd + 2] partial O (unnormalised), max (log2 units), sum
+	int* jobs;                     // [workers][kAcJobInts]: the item that a worker begins and others end
+};
+
+// One job: row0 and rows in q, first head, last worker of the item (0 rows: none).
+enum AcJob : int { kAcJobSeq = 0, kAcJobHead = 1, kAcJobRow = 2, kAcJobRows = 3, kAcJobLast = 4, kAcJobInts = 8 };
+
+struct AcSeq {
+	int row0, n, ctx, slot; // first row of q, rows, positions, slot
+};
+
+// Sequence s, with its numbers checked; n = 0 if it is empty, refused or not of this launch.
+__device__ __forceinline__ AcSeq ac_seq(const AttnChunkArgs& a, int s, bool report)
+{
+	AcSeq q;
+	const int b = a.q_start[s], e = a.q_start[s + 1];
+	q.row0 = b;
+	q.n = 0;
+	q.ctx = a.ctx_len[s];
+	q.slot = a.seq_slot ? a.seq_slot[s] : s;
+	if (e == b) return q;
+	int bad = 0;
+	if (b < 0 || e < b || e > a.n_tokens || e - b > a.max_new) bad = kDevBadIndex;
+	else if (q.slot < 0 || q.slot >= a.n_slots || q.ctx < 0 || q.ctx > a.pages_per_seq * a.blk) bad = kDevKvRange;
+	if (bad) {
+		if (report) report_err(a.status, bad);
+		return q;
+	}
+	const int64_t rows = (int64_t)(e - b) * a.G;
+	if (rows > a.rows_min && rows <= a.rows_max) q.n = e - b;
+	return q;
+}
+
+// The key tiles of rows [r0, r1) of a sequence: [0, sink) and [first, end); cost >= 1 so that a tile that
+// sees nothing is visited (its rows are zeros).
+struct AcTiles {
+	int lo;    // first position that the window of the tile's first row reaches
+	int hi;    // one past the last row's position (<= 0: none)
+	int sink, first, end, cost;
+};
+
+template <int KT>
+__device__ __forceinline__ AcTiles ac_tiles(const AttnChunkArgs& a, const AcSeq& q, int r0, int r1)
+{
+	AcTiles t;
+	const int p0 = q.ctx - q.n + r0 / a.G, p1 = q.ctx - q.n + (r1 - 1) / a.G;
+	t.hi = p1 + 1;
+	t.lo = a.window ? max(0, p0 - a.window + 1) : 0;
+	const int sinks = min(min(a.n_sink, t.lo), max(t.hi, 0)); // sinks below the window
+	t.end = t.hi > 0 ? (t.hi + KT - 1) / KT : 0;
+	t.first = min(t.lo / KT, t.end);
+	t.sink = min((sinks + KT - 1) / KT, t.first);
+	t.cost = max(1, t.sink + t.end - t.first);
+	return t;
+}
+// key tile i (0 .. cost - 1) of an item
+__device__ __forceinline__ int ac_tile_at(const AcTiles& t, int i) { return i < t.sink ? i : t.first + i - t.sink; }
+
+// Whether a row at position p sees key k (<= the context).
+__device__ __forceinline__ bool ac_sees(const AttnChunkArgs& a, int p, int k)
+{
+	return k <= p && (a.window == 0 || k > p - a.window || k < a.n_sink);
+}
+
+template <int R, int KT>
+__device__ __forceinline__ int ac_tile_cost(const AttnChunkArgs& a, const AcSeq& q, int tile)
+{
+	return ac_tiles<KT>(a, q, tile * R, min((tile + 1) * R, q.n * a.G)).cost;
+}
+
+// pre[s] = cost of the sequences before s over all heads, pre[n_seqs] = the total.  Every thread of the
+// CTA calls it (blockDim a multiple of 32, at most 1024); ends with a barrier.
+template <int R, int KT>
+__device__ __forceinline__ void ac_prefix(const AttnChunkArgs& a, uint32_t* pre)
+{
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+	const bool report = blockIdx.x == 0;
+	// a lane per sequence when tiles are few; a warp per sequence, its lanes over the tiles, otherwise
+	if (a.max_new * (int64_t)a.G <= 4 * R) {
+		for (int s = threadIdx.x; s < a.n_seqs; s += blockDim.x) {
+			const AcSeq q = ac_seq(a, s, report);
+			uint32_t c = 0;
+			for (int t = 0; t * R < q.n * a.G; ++t) c += ac_tile_cost<R, KT>(a, q, t);
+			pre[s + 1] = c * (uint32_t)a.KV;
+		}
+	} else {
+		for (int s = warp; s < a.n_seqs; s += warps) {
+			const AcSeq q = ac_seq(a, s, report && lane == 0);
+			const int tiles = (q.n * a.G + R - 1) / R;
+			uint32_t c = 0;
+			for (int t = lane; t < tiles; t += kWarp) c += ac_tile_cost<R, KT>(a, q, t);
+#pragma unroll
+			for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
+			if (lane == 0) pre[s + 1] = c * (uint32_t)a.KV;
+		}
+	}
+	if (threadIdx.x == 0) pre[0] = 0;
+	__syncthreads();
+	if (warp == 0) {
+		uint32_t carry = 0;
+		for (int base = 0; base < a.n_seqs; base += kWarp) {
+			const int s = base + lane;
+			uint32_t v = s < a.n_seqs ? pre[s + 1] : 0u;
+#pragma unroll
+			for (int o = 1; o < 32; o <<= 1) {
+				const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, v, o);
+				if (lane >= o) v += y;
+			}
+			if (s < a.n_seqs) pre[s + 1] = carry + v;
+			carry += __shfl_sync(0xFFFFFFFFu, v, 31);
+		}
+	}
+	__syncthreads();
+}
+
+// A worker's run of the laid-out costs, walked item by item (every lane of the warp holds the same).
+template <int R, int KT>
+struct AcRun {
+	uint32_t at, end, run; // position and end of the run, length of every run
+	int s, h, tile, tiles;
+	AcSeq q;
+	AcTiles t;
+	uint32_t item;         // where the current item begins
+
+	__device__ __forceinline__ bool done() const { return at >= end; }
+	// this worker's key tiles of the item: [from, to)
+	__device__ __forceinline__ int from() const { return (int)(at - item); }
+	__device__ __forceinline__ int to() const { return (int)(min(end, item + (uint32_t)t.cost) - item); }
+	__device__ __forceinline__ bool whole() const { return from() == 0 && to() == t.cost; }
+	__device__ __forceinline__ int rows() const { return min(R, q.n * g_ - tile * R); }
+	// slot of the partial: a worker ends at most one item that began before it and begins at most one
+	// that ends after it
+	__device__ __forceinline__ int slot(int worker) const { return 2 * worker + (from() == 0 ? 1 : 0); }
+	__device__ __forceinline__ int last_worker() const { return (int)((item + (uint32_t)t.cost - 1) / run); }
+	int g_;
+
+	__device__ __forceinline__ void tile_of(const AttnChunkArgs& a)
+	{
+		t = ac_tiles<KT>(a, q, tile * R, min((tile + 1) * R, q.n * a.G));
+	}
+
+	// by a whole warp
+	__device__ __forceinline__ void begin(const AttnChunkArgs& a, const uint32_t* pre, int worker)
+	{
+		const int lane = threadIdx.x & 31;
+		const uint32_t total = pre[a.n_seqs];
+		run = max((uint32_t)a.min_run, (total + (uint32_t)a.workers - 1) / (uint32_t)a.workers);
+		const uint64_t b = (uint64_t)run * (uint32_t)worker;
+		at = b < total ? (uint32_t)b : total;
+		end = (uint32_t)min(b + run, (uint64_t)total);
+		g_ = a.G;
+		if (done()) return;
+		int l = 0, r = a.n_seqs; // the last s with pre[s] <= at
+		while (r - l > 1) {
+			const int m = (l + r) >> 1;
+			if (pre[m] <= at) l = m;
+			else r = m;
+		}
+		s = l;
+		q = ac_seq(a, s, false);
+		tiles = (q.n * a.G + R - 1) / R;
+		const uint32_t per_head = (pre[s + 1] - pre[s]) / (uint32_t)a.KV;
+		const uint32_t in = at - pre[s];
+		h = (int)(in / per_head);
+		uint32_t left = in % per_head;
+		item = at - left;
+		// the tile that holds `left`: 32 tiles at a time
+		for (tile = 0;; tile += kWarp) {
+			const int my = tile + lane;
+			const uint32_t c = my < tiles ? (uint32_t)ac_tile_cost<R, KT>(a, q, my) : 0u;
+			uint32_t x = c;
+#pragma unroll
+			for (int o = 1; o < 32; o <<= 1) {
+				const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+				if (lane >= o) x += y;
+			}
+			const unsigned hit = __ballot_sync(0xFFFFFFFFu, x > left);
+			const uint32_t all = __shfl_sync(0xFFFFFFFFu, x, 31);
+			if (hit) {
+				const int k = __ffs(hit) - 1;
+				item += __shfl_sync(0xFFFFFFFFu, x - c, k);
+				tile += k;
+				break;
+			}
+			left -= all;
+			item += all;
+		}
+		tile_of(a);
+	}
+
+	__device__ __forceinline__ void next(const AttnChunkArgs& a, const uint32_t* pre)
+	{
+		item += (uint32_t)t.cost;
+		at = item;
+		if (done()) return;
+		if (++tile == tiles) {
+			tile = 0;
+			if (++h == a.KV) {
+				h = 0;
+				do ++s;
+				while (pre[s + 1] == pre[s]);
+				q = ac_seq(a, s, false);
+				tiles = (q.n * a.G + R - 1) / R;
+			}
+		}
+		tile_of(a);
+	}
+};
+
+// The record of an item that worker `w` begins and does not end (one lane calls it), or of none.
+template <int R, int KT>
+__device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w, const AcRun<R, KT>* run)
+{
+	int* j = a.jobs + (size_t)w * kAcJobInts;
+	if (!run) {
+		j[kAcJobRows] = 0;
+		return;
+	}
+	j[kAcJobSeq] = run->q.row0;
+	j[kAcJobHead] = run->h;
+	j[kAcJobRow] = run->tile * R;
+	j[kAcJobRows] = run->rows();
+	j[kAcJobLast] = run->last_worker();
+}
+
+// floats of one partial: R rows of O, each row's max and sum
+__host__ __device__ constexpr size_t ac_part_floats(int R, int hd) { return (size_t)R * (hd + 2); }
+
+// Joins the shares of every item that a cut divides: blockIdx.x is the worker that began it, blockIdx.y a
+// block of rows.  A partial holds O as [hd / 4][R] float4 when `columns`, else [R][hd], then the rows'
+// max and sum.
+//   m = max_i m_i,  O = sum_i 2^(m_i - m) O_i,  l = sum_i 2^(m_i - m) l_i,  out = O / l
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_chunk_combine(const AttnChunkArgs a, int R, int columns)
+{
+	pdl_wait();
+	pdl_trigger();
+	const int w0 = blockIdx.x;
+	const int* j = a.jobs + (size_t)w0 * kAcJobInts;
+	const int rows = j[kAcJobRows];
+	if (rows == 0) return;
+	const int last = j[kAcJobLast], hd4 = a.hd / 4;
+	const size_t pf = ac_part_floats(R, a.hd);
+	const float* first = a.part + (size_t)(2 * w0 + 1) * pf; // the beginner's share; the others' are slot 2 w
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+	for (int r = blockIdx.y * warps + warp; r < rows; r += gridDim.y * warps) {
+		auto part = [&](int w) { return w == w0 ? first : a.part + (size_t)(2 * w) * pf; };
+		float m = -INFINITY;
+		for (int w = w0 + lane; w <= last; w += kWarp) m = fmaxf(m, part(w)[(size_t)R * a.hd + r]);
+		m = warp_max(m);
+		float l = 0.0f;
+		for (int w = w0 + lane; w <= last; w += kWarp) {
+			const float* p = part(w) + (size_t)R * a.hd;
+			l += p[r] == -INFINITY ? 0.0f : exp2f(p[r] - m) * p[R + r];
+		}
+		l = warp_sum(l);
+		const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+		const int fr = j[kAcJobRow] + r;
+		T* out = reinterpret_cast<T*>(a.out) + (size_t)(j[kAcJobSeq] + fr / a.G) * a.out_stride +
+		         (size_t)(j[kAcJobHead] * a.G + fr % a.G) * a.hd;
+		for (int c = lane; c < hd4; c += kWarp) {
+			float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+			for (int w = w0; w <= last; ++w) {
+				const float* p = part(w);
+				const float mw = p[(size_t)R * a.hd + r];
+				const float f = mw == -INFINITY ? 0.0f : exp2f(mw - m);
+				const float4 v = reinterpret_cast<const float4*>(p)[columns ? (size_t)c * R + r : (size_t)r * hd4 + c];
+				if (f == 0.0f) continue; // a share without keys may hold anything
+				o.x = fmaf(f, v.x, o.x);
+				o.y = fmaf(f, v.y, o.y);
+				o.z = fmaf(f, v.z, o.z);
+				o.w = fmaf(f, v.w, o.w);
+			}
+			Store<T>::put(out + 4 * c, o.x * inv);
+			Store<T>::put(out + 4 * c + 1, o.y * inv);
+			Store<T>::put(out + 4 * c + 2, o.z * inv);
+			Store<T>::put(out + 4 * c + 3, o.w * inv);
+		}
+	}
+}
+
+// ---- the fp32 kernel ------------------------------------------------------------------
+// Every type, head size, group and page size; a CTA of four warps is a worker.  Tiles of 16 rows x 32
+// keys: K and V rows go to shared memory as fp32, a lane owns a key for the scores (four rows of its
+// warp at a time) and head dims for P.V.  Bound by shared-memory reads: per key and four head dims one
+// 16-byte read of K and one of every row's q for 16 FMAs.  It serves the fp32 decoder (head_dim 48) and
+// what the tensor-core kernels do not take.
+constexpr int kAfR = 16;
+constexpr int kAfKT = 32;
+constexpr int kAfThreads = 128;
+constexpr int kAfRows = kAfR / (kAfThreads / kWarp); // rows per warp
+
+// q [16][hd], K or V [32][hd + 4], P [16][32]
+__host__ __device__ constexpr size_t attn_chunk_f32_smem(int hd, int n_seqs)
+{
+	return ((size_t)kAfR * hd + (size_t)kAfKT * (hd + 4) + kAfR * kAfKT) * 4 + (size_t)(n_seqs + 1) * 4;
+}
+
+// VPL: groups of 4 head dims per lane (head_dim <= 128 VPL)
+template <typename T, int VPL>
+__global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkArgs a)
+{
+	extern __shared__ __align__(16) float af_smem[];
+	pdl_wait();
+	pdl_trigger();
+	const int hd = a.hd, ld = hd + 4, hd4 = hd / 4;
+	float* q_s = af_smem;                 // [16][hd], scaled to log2 units
+	float* kv_s = q_s + kAfR * hd;        // [32][ld]
+	float* p_s = kv_s + kAfKT * ld;       // [16][32]
+	uint32_t* pre = reinterpret_cast<uint32_t*>(p_s + kAfR * kAfKT);
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, worker = blockIdx.x;
+	ac_prefix<kAfR, kAfKT>(a, pre);
+	AcRun<kAfR, kAfKT> run;
+	run.begin(a, pre, worker);
+	if (threadIdx.x == 0) ac_job<kAfR, kAfKT>(a, worker, nullptr);
+	const float sl2 = a.scale * 1.4426950408889634f;
+	constexpr int V = Store<T>::kVec;
+	for (; !run.done(); run.next(a, pre)) {
+		const int rows = run.rows(), r0 = run.tile * kAfR;
+		const AcTiles t = run.t;
+		const int base_pos = run.q.ctx - run.q.n;
+		__syncthreads(); // q_s is free
+		for (int u = threadIdx.x; u < kAfR * (hd / V); u += kAfThreads) {
+			const int r = u / (hd / V), c = u % (hd / V);
+			float f[V];
+			uint4 v = make_uint4(0, 0, 0, 0);
+			if (r < rows) {
+				const int fr = r0 + r;
+				v = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (size_t)(run.q.row0 + fr / a.G) * a.q_stride +
+				                                   (size_t)(run.h * a.G + fr % a.G) * hd)[c];
+			}
+			unpack_unit(v, f, (const T*)nullptr);
+#pragma unroll
+			for (int i = 0; i < V; ++i) q_s[r * hd + c * V + i] = f[i] * sl2;
+		}
+		float4 o[kAfRows][VPL];
+		float m[kAfRows], l[kAfRows];
+		int pos[kAfRows];
+#pragma unroll
+		for (int i = 0; i < kAfRows; ++i) {
+			m[i] = -INFINITY;
+			l[i] = 0.0f;
+			const int r = warp * kAfRows + i;
+			pos[i] = r < rows ? base_pos + (r0 + r) / a.G : -1;
+#pragma unroll
+			for (int v = 0; v < VPL; ++v) o[i][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+		}
+		for (int kt = run.from(); kt < run.to(); ++kt) {
+			const int k0 = ac_tile_at(t, kt) * kAfKT;
+			// one pool's 32 rows of the tile; rows that no row of the item sees are zeros, so that nothing
+			// they hold reaches a sum
+			auto stage = [&](const void* pool) {
+				for (int u = threadIdx.x; u < kAfKT * (hd / V); u += kAfThreads) {
+					const int k = k0 + u / (hd / V), c = u % (hd / V);
+					uint4 x = make_uint4(0, 0, 0, 0);
+					if (k < t.hi && (k >= t.lo || k < a.n_sink)) {
+						const int page = a.table[(size_t)run.q.slot * a.pages_per_seq + k / a.blk];
+						if (page >= 0 && page < a.n_pages)
+							x = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(pool) +
+							                                   (((size_t)page * a.KV + run.h) * a.blk + k % a.blk) * hd)[c];
+						else
+							report_err(a.status, kDevKvRange);
+					}
+					float f[V];
+					unpack_unit(x, f, (const T*)nullptr);
+#pragma unroll
+					for (int i = 0; i < V; i += 4)
+						*reinterpret_cast<float4*>(kv_s + (size_t)(k - k0) * ld + c * V + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+				}
+			};
+			__syncthreads();
+			stage(a.kpool);
+			__syncthreads();
+			float sc[kAfRows];
+#pragma unroll
+			for (int i = 0; i < kAfRows; ++i) sc[i] = 0.0f;
+			for (int d = 0; d < hd; d += 4) {
+				const float4 kk = *reinterpret_cast<const float4*>(kv_s + (size_t)lane * ld + d);
+#pragma unroll
+				for (int i = 0; i < kAfRows; ++i) {
+					const float4 qq = *reinterpret_cast<const float4*>(q_s + (warp * kAfRows + i) * hd + d);
+					sc[i] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, sc[i]))));
+				}
+			}
+#pragma unroll
+			for (int i = 0; i < kAfRows; ++i) {
+				const bool sees = pos[i] >= 0 && ac_sees(a, pos[i], k0 + lane);
+				const float s = sees ? sc[i] : -INFINITY;
+				const float mn = fmaxf(m[i], warp_max(s));
+				// no key seen so far (mn -inf): weights and the factor are zero
+				const float f = m[i] == -INFINITY ? 0.0f : exp2f(m[i] - mn);
+				const float p = sees ? exp2f(s - mn) : 0.0f;
+				m[i] = mn;
+				l[i] = l[i] * f + warp_sum(p);
+				p_s[(warp * kAfRows + i) * kAfKT + lane] = p;
+#pragma unroll
+				for (int v = 0; v < VPL; ++v) {
+					o[i][v].x *= f;
+					o[i][v].y *= f;
+					o[i][v].z *= f;
+					o[i][v].w *= f;
+				}
+			}
+			__syncthreads(); // K is read, P written
+			stage(a.vpool);
+			__syncthreads();
+			for (int k = 0; k < kAfKT; k += 4) {
+				float4 p[kAfRows];
+#pragma unroll
+				for (int i = 0; i < kAfRows; ++i) p[i] = *reinterpret_cast<const float4*>(p_s + (warp * kAfRows + i) * kAfKT + k);
+#pragma unroll
+				for (int v = 0; v < VPL; ++v) {
+					const int c = lane + v * kWarp;
+					if (c >= hd4) continue;
+#pragma unroll
+					for (int kk = 0; kk < 4; ++kk) {
+						const float4 x = *reinterpret_cast<const float4*>(kv_s + (size_t)(k + kk) * ld + c * 4);
+#pragma unroll
+						for (int i = 0; i < kAfRows; ++i) {
+							const float w = kk == 0 ? p[i].x : kk == 1 ? p[i].y : kk == 2 ? p[i].z : p[i].w;
+							o[i][v].x = fmaf(w, x.x, o[i][v].x);
+							o[i][v].y = fmaf(w, x.y, o[i][v].y);
+							o[i][v].z = fmaf(w, x.z, o[i][v].z);
+							o[i][v].w = fmaf(w, x.w, o[i][v].w);
+						}
+					}
+				}
+			}
+		}
+		const bool whole = run.whole();
+		float* part = a.part + (size_t)run.slot(worker) * ac_part_floats(kAfR, hd);
+#pragma unroll
+		for (int i = 0; i < kAfRows; ++i) {
+			const int r = warp * kAfRows + i;
+			if (r >= rows) continue;
+			if (whole) {
+				const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
+				const int fr = r0 + r;
+				T* out = reinterpret_cast<T*>(a.out) + (size_t)(run.q.row0 + fr / a.G) * a.out_stride + (size_t)(run.h * a.G + fr % a.G) * hd;
+#pragma unroll
+				for (int v = 0; v < VPL; ++v) {
+					const int c = lane + v * kWarp;
+					if (c >= hd4) continue;
+					Store<T>::put(out + 4 * c, o[i][v].x * inv);
+					Store<T>::put(out + 4 * c + 1, o[i][v].y * inv);
+					Store<T>::put(out + 4 * c + 2, o[i][v].z * inv);
+					Store<T>::put(out + 4 * c + 3, o[i][v].w * inv);
+				}
+			} else {
+#pragma unroll
+				for (int v = 0; v < VPL; ++v) {
+					const int c = lane + v * kWarp;
+					if (c < hd4) reinterpret_cast<float4*>(part)[(size_t)r * hd4 + c] = o[i][v];
+				}
+				if (lane == 0) {
+					part[(size_t)kAfR * hd + r] = m[i];
+					part[(size_t)kAfR * hd + kAfR + r] = l[i];
+				}
+			}
+		}
+		if (!whole && run.from() == 0 && threadIdx.x == 0) ac_job<kAfR, kAfKT>(a, worker, &run);
+	}
+}
+
+} // namespace inf

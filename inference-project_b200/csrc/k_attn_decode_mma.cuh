@@ -23,7 +23,7 @@
 #include "common.cuh"
 #include "k_attn_decode.cuh"        // AttnDecodeArgs, AttnKernel, attn_vpl
 #include "k_attn_decode_stream.cuh" // kStChunkPages, kStBufs, attn_stream_splits
-#include "k_attn_prefill_tc.cuh"    // tma_load_4d (4-D boxes of the paged K/V pool)
+#include "tensor_core.cuh"          // tma_load_4d (4-D boxes of the paged K/V pool), mma, ldmatrix
 
 namespace inf {
 
@@ -45,32 +45,6 @@ inline size_t attn_mma_smem_bytes(int hd, int blk, int pages_per_seq)
 	       (kAmThreads / 32) * kStBufs * sizeof(uint64_t);
 }
 
-__device__ __forceinline__ void mma_bf16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-	asm volatile(
-	    "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-	    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-	    : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
-{
-	const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-	return *reinterpret_cast<const uint32_t*>(&b);
-}
-__device__ __forceinline__ uint32_t pack_raw_bf16(uint16_t lo, uint16_t hi) { return (uint32_t)lo | ((uint32_t)hi << 16); }
-
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3)
-{
-	asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-	             : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-	             : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3)
-{
-	asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-	             : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-	             : "r"(addr));
-}
 // Byte offset of 16-byte chunk c16 of row r (position) in half h of one page of K or V in
 // shared memory: [head_dim / 64 halves][16 positions][128 bytes], each half two SWIZZLE_128B
 // atoms (8 positions x 128 bytes) as the TMA box writes it.

@@ -21,7 +21,7 @@
 #pragma once
 
 #include "k_attn_prefill.cuh" // AttnPrefillArgs
-#include "k_gemm_tc.cuh"      // tma_load_2d, umma_bf16, umma_commit, tmem_ld_32cols, fences
+#include "tensor_core.cuh"    // tma_load_4d, umma_bf16, umma_commit, tmem_ld_32cols, fences
 
 namespace inf {
 
@@ -30,69 +30,6 @@ constexpr int kPtKeys = 128;       // keys per tile (MMA N of S, K of P.V)
 constexpr int kPtStages = 2;
 constexpr int kPtThreads = 320; // TMA warp, MMA warp, 8 softmax warps
 constexpr uint32_t kPtAtom = 128 * 64 * 2; // one [128 x 64] bf16 SWIZZLE_128B block: 16 KB
-
-// shared-memory descriptor with explicit leading / stride byte offsets (SWIZZLE_128B)
-__device__ __forceinline__ uint64_t umma_desc_sw128_lbo(uint32_t smem_addr, uint32_t lbo, uint32_t sbo)
-{
-	uint64_t d = 0;
-	d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-	d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
-	d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
-	d |= (uint64_t)1u << 46;
-	d |= (uint64_t)2u << 61;
-	return d;
-}
-
-// tcgen05.ld of 32 columns without the wait (several loads, then one tcgen05.wait::ld)
-__device__ __forceinline__ void tmem_ld_32cols_nowait(uint32_t taddr, float* v)
-{
-	uint32_t r[32];
-	asm volatile(
-	    "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-	    "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-	    "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-	    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-	      "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-	      "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-	      "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-	    : "r"(taddr));
-#pragma unroll
-	for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-__device__ __forceinline__ void tmem_st_32cols(uint32_t taddr, const float (&v)[32])
-{
-	uint32_t r[32];
-#pragma unroll
-	for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
-	asm volatile(
-	    "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-	    "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-	    "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-	    "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-	    "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-	    "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-	    "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-	    : "memory");
-	asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// 4-D tiled TMA load (head_dim, row in page, KV head, page) of the paged K/V pool
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar,
-                                            uint64_t policy)
-{
-	asm volatile(
-	    "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-	    " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(smem_u32(dst)),
-	    "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)), "l"(policy)
-	    : "memory");
-}
-
-// byte offset of 16-byte chunk c (0..7) of row r inside a SWIZZLE_128B block of 128-byte rows
-__device__ __forceinline__ uint32_t sw128_off(int r, int c)
-{
-	return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
-}
 
 struct PtLayout {
 	size_t q, k, v, p, bars, total;
@@ -112,13 +49,6 @@ __host__ __device__ inline PtLayout pt_layout(int hd)
 	return L;
 }
 inline size_t attn_prefill_tc_smem_bytes(int hd) { return 1024 + pt_layout(hd).total; }
-
-__device__ __forceinline__ float ex2_approx(float x)
-{
-	float y;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-	return y;
-}
 
 // Largest growth of the running max (log2 units) absorbed without rescaling O: P values up to
 // 2^8 stay exact enough in bf16 and fp32, and O / l is unchanged in exact arithmetic.

@@ -24,6 +24,7 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "tensor_core.cuh"
 
 namespace inf {
 
@@ -71,70 +72,6 @@ struct TcArgs {
 	// would leave SMs idle
 	int bn;
 };
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar, uint64_t policy)
-{
-	asm volatile(
-	    "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-	    " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_u32(dst)),
-	    "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)), "l"(policy)
-	    : "memory");
-}
-
-// K-major operand in the canonical SWIZZLE_128B layout: 8-row atoms of 1024 bytes stacked
-// along M/N (stride byte offset 1024), version 1 (sm_100), layout type 2 (128B swizzle).
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr)
-{
-	uint64_t d = 0;
-	d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-	d |= (uint64_t)1u << 16;               // leading byte offset (unused for swizzled K-major): 16 B
-	d |= (uint64_t)(1024u >> 4) << 32;     // stride byte offset: 1024 B between 8-row atoms
-	d |= (uint64_t)1u << 46;               // descriptor version for sm_100
-	d |= (uint64_t)2u << 61;               // SWIZZLE_128B
-	return d;
-}
-
-// kind::f16 instruction descriptor: D f32, A/B bf16, both K-major, M = 128, N = 256.
-__host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N)
-{
-	return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
-{
-	asm volatile(
-	    "{\n\t.reg .pred p;\n\t"
-	    "setp.ne.b32 p, %4, 0;\n\t"
-	    "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-	    "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-	    : "memory");
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t* bar)
-{
-	asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-	             : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld_32cols(uint32_t taddr, float (&v)[32])
-{
-	uint32_t r[32];
-	asm volatile(
-	    "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-	    "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-	    "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-	    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-	      "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-	      "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-	      "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-	    : "r"(taddr));
-	asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-	for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // The fused epilogues, one output column per lane: the whole warp calls it for token row t
 // and columns n = n0 + lane (n0 a multiple of 32).  The column pairs of the

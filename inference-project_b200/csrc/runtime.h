@@ -1,6 +1,7 @@
 // Host-side helpers shared by the translation units of libinf.so.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdarg>
@@ -27,6 +28,16 @@ Error_t fail(Error_t err, const char* fmt, ...);
 	} while (0)
 
 bool is_device_ptr(const void* p);
+// Whether p is memory the current device's kernels may be given: device memory of that device, or
+// managed memory.
+bool is_local_device_ptr(const void* p);
+
+// The Error_t of a device error word (DevErr), with its description recorded.
+Error_t map_dev_err(int v);
+
+// A layer's paged K or V pool [pages][KV][blk][hd] as a 4-D tensor (hd, row, head, page) with boxes
+// of 64 head dims x box_rows rows (0: blk) x 1 head x box_pages pages, SWIZZLE_128B.
+Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages, u32 box_rows = 0);
 
 // Whether inf_set_sampling turned sampling on for this model (false for NULL).
 bool model_sampling_on(const Model* m);

@@ -76,6 +76,25 @@ class Model(C.Structure):
     _fields_ = [("config", InfConfig), ("data", vp), ("model_bsize", u64), ("engine", vp)]
 
 
+class InfPagedKv(C.Structure):
+    _fields_ = [("kpool", vp), ("vpool", vp), ("block_table", vp), ("page_refs", vp), ("layer_stride", u64),
+                ("n_layers", u32), ("n_slots", u32), ("pages_per_seq", u32), ("n_pages", u32), ("n_kv_heads", u32),
+                ("head_dim", u32), ("kv_block", u32), ("dtype", u32)]
+
+
+class InfQkNormRope(C.Structure):
+    _fields_ = [("qkv", vp), ("q_out", vp), ("qkv_stride", u64), ("q_out_stride", u64), ("q_gain", vp), ("k_gain", vp),
+                ("rope_cos", vp), ("rope_sin", vp), ("tok_slot", vp), ("tok_pos", vp), ("status", vp), ("eps", f32),
+                ("gain_offset", f32), ("n_pos", u32), ("n_tokens", u32), ("n_heads", u32), ("layer", u32)]
+
+
+class InfAttnChunk(C.Structure):
+    _fields_ = [("q", vp), ("out", vp), ("q_stride", u64), ("out_stride", u64), ("q_start", vp), ("ctx_len", vp),
+                ("seq_slot", vp), ("scratch", vp), ("scratch_bytes", u64), ("status", vp), ("scale", f32),
+                ("n_seqs", u32), ("n_tokens", u32), ("max_new", u32), ("n_heads", u32), ("window", u32),
+                ("n_sink", u32), ("layer", u32)]
+
+
 class InfStats(C.Structure):
     _fields_ = [("prefill_ms", f64), ("decode_ms", f64), ("n_prompt", u32), ("n_new", u32),
                 ("kernel_launches", u64)]
@@ -87,7 +106,9 @@ EXPORTS = [
     "arena_dev_push", "arena_dev_pop", "arena_dev_pop_at", "arena_dev_pos_get", "cu_malloc", "cu_free",
     "cu_memcpy_htd", "cu_memcpy_htd_async", "cu_memcpy_dth", "cu_host_register_read_only", "cu_memset",
     "inf_fetch_input_embeddings", "inf_rmsnorm", "inf_gemm_bf16", "inf_attn_decode_scratch_bytes", "inf_attn_decode",
-    "inf_attn_decode_with", "inf_attn_prefill",
+    "inf_attn_decode_with", "inf_attn_prefill", "inf_check_status", "inf_qk_norm_rope", "inf_attn_chunk",
+    "inf_attn_chunk_scratch_bytes", "inf_kv_copy_pages", "inf_kv_free", "inf_kv_fork", "inf_kv_compact",
+    "inf_kv_pages_scratch_bytes",
     "inf_config_preset", "inf_model_build", "inf_model_destroy", "inf_forward", "inf_forward_batch",
     "inf_generate", "inf_decode", "inf_seq_reset", "inf_error_string", "inf_last_error_detail", "inf_model_stream",
     "inf_kernel_launches", "inf_batch_h2d_bytes", "inf_decode_bytes", "inf_profile_decode_step", "inf_synth_ids", "inf_debug_read",
@@ -143,6 +164,15 @@ def lib():
         "inf_attn_decode_with": (E, [u32, vp, vp, vp, vp, u32, u32, vp, vp, u32, u32, u32, u32, u32, u32, vp, vp, u64,
                                      vp]),
         "inf_attn_prefill": (E, [u32, vp, vp, vp, vp, u32, u32, vp, vp, u32, u32, u32, u32, u32, vp, vp]),
+        "inf_check_status": (E, [vp, vp]),
+        "inf_qk_norm_rope": (E, [C.POINTER(InfPagedKv), C.POINTER(InfQkNormRope), vp]),
+        "inf_attn_chunk": (E, [C.POINTER(InfPagedKv), C.POINTER(InfAttnChunk), vp]),
+        "inf_attn_chunk_scratch_bytes": (u64, [C.POINTER(InfPagedKv), u32, u32, u32]),
+        "inf_kv_copy_pages": (E, [C.POINTER(InfPagedKv), vp, vp, u32, vp, vp]),
+        "inf_kv_free": (E, [C.POINTER(InfPagedKv), vp, vp, vp, u32, vp, vp]),
+        "inf_kv_fork": (E, [C.POINTER(InfPagedKv), vp, vp, vp, u32, vp, u64, vp, vp]),
+        "inf_kv_compact": (E, [C.POINTER(InfPagedKv), vp, vp, vp, u64, vp, vp]),
+        "inf_kv_pages_scratch_bytes": (u64, [C.POINTER(InfPagedKv)]),
         "inf_config_preset": (E, [u32, C.POINTER(InfConfig)]),
         "inf_model_build": (E, [C.POINTER(C.POINTER(ExecCtx)), C.POINTER(Model), C.POINTER(InfConfig), C.c_char_p, u64]),
         "inf_model_destroy": (E, [C.POINTER(C.POINTER(ExecCtx)), C.POINTER(Model)]),
@@ -595,6 +625,81 @@ def attn_decode_noalloc(d_q, d_k, d_v, d_bt, pages_per_seq, n_pages, d_slot, d_p
     check(lib().inf_attn_decode_noalloc(vp(d_q), vp(d_k), vp(d_v), vp(d_bt), pages_per_seq, n_pages, vp(d_slot),
                                         vp(d_pos), n_tokens, n_heads, n_kv_heads, head_dim, kv_block, dtype,
                                         vp(d_out), vp(stream) if stream else None), "inf_attn_decode_noalloc")
+
+
+# ---- a paged KV cache of the caller's (device pointers as ints, 0: NULL) ----------------------
+# The descriptors below are built once beside the cache and its buffers and passed to every call.
+
+def paged_kv(d_kpool, d_vpool, *, n_pages, n_kv_heads, head_dim, kv_block, dtype, d_block_table=0, n_slots=0,
+             pages_per_seq=0, d_page_refs=0, n_layers=1, layer_stride=0) -> InfPagedKv:
+    return InfPagedKv(kpool=d_kpool, vpool=d_vpool, block_table=d_block_table, page_refs=d_page_refs,
+                      layer_stride=layer_stride, n_layers=n_layers, n_slots=n_slots, pages_per_seq=pages_per_seq,
+                      n_pages=n_pages, n_kv_heads=n_kv_heads, head_dim=head_dim, kv_block=kv_block, dtype=dtype)
+
+
+def check_status(d_status: int, stream: int = 0) -> None:
+    """Waits for the stream; raises the failure the status word holds and clears it."""
+    check(lib().inf_check_status(d_status, stream or None), "inf_check_status")
+
+
+def qk_norm_rope_args(*, d_qkv, d_q_out, d_cos, d_sin, n_pos, d_tok_slot, d_tok_pos, n_tokens, n_heads, d_q_gain=0,
+                      d_k_gain=0, eps=1e-6, gain_offset=0.0, qkv_stride=0, q_out_stride=0, layer=0,
+                      d_status=0) -> InfQkNormRope:
+    return InfQkNormRope(qkv=d_qkv, q_out=d_q_out, qkv_stride=qkv_stride, q_out_stride=q_out_stride, q_gain=d_q_gain,
+                         k_gain=d_k_gain, rope_cos=d_cos, rope_sin=d_sin, tok_slot=d_tok_slot, tok_pos=d_tok_pos,
+                         status=d_status, eps=eps, gain_offset=gain_offset, n_pos=n_pos, n_tokens=n_tokens,
+                         n_heads=n_heads, layer=layer)
+
+
+def qk_norm_rope(kv: InfPagedKv, args: InfQkNormRope, stream: int = 0) -> None:
+    """Norm and rotation of new tokens' queries and keys, queries out, keys and values into the cache."""
+    rc = lib().inf_qk_norm_rope(kv, args, stream or None)
+    if rc:
+        check(rc, "inf_qk_norm_rope")
+
+
+def attn_chunk_scratch_bytes(kv: InfPagedKv, *, n_heads, n_tokens, n_seqs) -> int:
+    return int(lib().inf_attn_chunk_scratch_bytes(kv, n_heads, n_tokens, n_seqs))
+
+
+def attn_chunk_args(*, d_q, d_out, d_q_start, d_ctx_len, n_seqs, n_tokens, n_heads, d_scratch, scratch_bytes,
+                    max_new=0, d_seq_slot=0, window=0, n_sink=0, scale=0.0, q_stride=0, out_stride=0, layer=0,
+                    d_status=0) -> InfAttnChunk:
+    return InfAttnChunk(q=d_q, out=d_out, q_stride=q_stride, out_stride=out_stride, q_start=d_q_start,
+                        ctx_len=d_ctx_len, seq_slot=d_seq_slot, scratch=d_scratch, scratch_bytes=scratch_bytes,
+                        status=d_status, scale=scale, n_seqs=n_seqs, n_tokens=n_tokens, max_new=max_new,
+                        n_heads=n_heads, window=window, n_sink=n_sink, layer=layer)
+
+
+def attn_chunk(kv: InfPagedKv, args: InfAttnChunk, stream: int = 0) -> None:
+    """Attention of a ragged batch of new tokens over the paged cache."""
+    rc = lib().inf_attn_chunk(kv, args, stream or None)
+    if rc:
+        check(rc, "inf_attn_chunk")
+
+
+def kv_copy_pages(kv: InfPagedKv, d_src, d_dst, n, d_status=0, stream=0) -> None:
+    check(lib().inf_kv_copy_pages(kv, d_src or None, d_dst or None, n, d_status or None, stream or None),
+          "inf_kv_copy_pages")
+
+
+def kv_free(kv: InfPagedKv, d_slot, d_first, d_last, n, d_status=0, stream=0) -> None:
+    check(lib().inf_kv_free(kv, d_slot or None, d_first or None, d_last or None, n, d_status or None, stream or None),
+          "inf_kv_free")
+
+
+def kv_pages_scratch_bytes(kv: InfPagedKv) -> int:
+    return int(lib().inf_kv_pages_scratch_bytes(kv))
+
+
+def kv_fork(kv: InfPagedKv, d_src, d_dst, d_len, n, d_scratch, scratch_bytes, d_status=0, stream=0) -> None:
+    check(lib().inf_kv_fork(kv, d_src or None, d_dst or None, d_len or None, n, d_scratch or None, scratch_bytes,
+                            d_status or None, stream or None), "inf_kv_fork")
+
+
+def kv_compact(kv: InfPagedKv, d_map, d_n_live, d_scratch, scratch_bytes, d_status=0, stream=0) -> None:
+    check(lib().inf_kv_compact(kv, d_map or None, d_n_live or None, d_scratch or None, scratch_bytes, d_status or None,
+                               stream or None), "inf_kv_compact")
 
 
 def rmsnorm(d_x: int, d_y: int, rows: int, dim: int, d_gain: int, eps: float, dtype: int, stream: int = 0) -> None:
