@@ -6,6 +6,7 @@
 #include <cstring>
 
 #include "k_attn_chunk.cuh"
+#include "k_attn_chunk_tc.cuh"
 #include "launch.h"
 
 using namespace inf;
@@ -16,10 +17,10 @@ u64 up256(u64 n) { return (n + 255) & ~255ull; }
 
 // One kernel's share of a call: the sequences with rows_min < rows <= rows_max rows per KV head.
 struct ChunkPass {
-	enum Kind { F32 } kind;
+	enum Kind { F32, TC } kind;
 	int rows_min, rows_max;
 	int workers, min_run;
-	int R, columns;      // row tile and layout of the partials
+	int R;               // row tile
 	size_t smem;
 	u64 part_off, jobs_off;
 };
@@ -62,6 +63,17 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 		P->pass[P->n_pass++] = p;
 		return Success;
 	};
+	const u32 blk = kv->kv_block;
+	if (kv->dtype == InfBF16 && (kv->head_dim == 64 || kv->head_dim == 128) && (blk == 16 || blk == 32 || blk == 64 || blk == 128)) {
+		ChunkPass t = {};
+		t.kind = ChunkPass::TC;
+		t.rows_max = 0x7FFFFFFF;
+		t.R = kCtR;
+		t.min_run = 2;
+		t.smem = ct_layout((int)kv->head_dim, (int)n_seqs).total;
+		t.workers = sms;
+		return add(t, units_max(kv, n_heads, n_tokens, n_seqs, kCtR, kCtKT));
+	}
 	ChunkPass f = {};
 	f.kind = ChunkPass::F32;
 	f.rows_max = 0x7FFFFFFF;
@@ -78,6 +90,19 @@ Error_t launch_f32(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
 	void (*k)(const AttnChunkArgs) = a.hd <= 128 ? k_attn_chunk_f32<T, 1> : a.hd <= 256 ? k_attn_chunk_f32<T, 2> : k_attn_chunk_f32<T, 4>;
 	INF_TRY(allow_smem(k, attn_chunk_f32_smem(a.hd <= 128 ? 128 : a.hd <= 256 ? 256 : 512, kAcMaxSeqs)));
 	return launch_pdl(k, dim3((unsigned)p.workers), dim3(kAfThreads), p.smem, st, a);
+}
+
+template <int HD>
+Error_t launch_tc(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
+{
+	const u32 blk = (u32)a.blk, box = kCtKT / blk;
+	CUtensorMap k8, k1, v8, v1;
+	INF_TRY(tensor_map_kv(&k8, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
+	INF_TRY(tensor_map_kv(&k1, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
+	INF_TRY(tensor_map_kv(&v8, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
+	INF_TRY(tensor_map_kv(&v1, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
+	INF_TRY(allow_smem(k_attn_chunk_tc<HD>, 227 * 1024));
+	return launch_pdl(k_attn_chunk_tc<HD>, dim3((unsigned)p.workers), dim3(kCtThreads), p.smem, st, k8, k1, v8, v1, a);
 }
 
 } // namespace
@@ -157,14 +182,15 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 	};
 	for (int i = 0; i < P.n_pass; ++i) {
 		const AttnChunkArgs b = pass_args(P.pass[i]);
-		INF_TRY(kv->dtype == InfBF16 ? launch_f32<bf16>(b, P.pass[i], st) : launch_f32<float>(b, P.pass[i], st));
+		if (P.pass[i].kind == ChunkPass::TC) INF_TRY(a.hd == 64 ? launch_tc<64>(b, P.pass[i], st) : launch_tc<128>(b, P.pass[i], st));
+		else INF_TRY(kv->dtype == InfBF16 ? launch_f32<bf16>(b, P.pass[i], st) : launch_f32<float>(b, P.pass[i], st));
 	}
 	for (int i = 0; i < P.n_pass; ++i) {
 		const ChunkPass& p = P.pass[i];
 		const AttnChunkArgs b = pass_args(p);
 		const dim3 grid((unsigned)p.workers, (unsigned)((p.R + 31) / 32));
-		INF_TRY(launch_pdl(kv->dtype == InfBF16 ? k_attn_chunk_combine<bf16> : k_attn_chunk_combine<float>, grid, dim3(256), 0, st, b,
-		                   p.R, p.columns));
+		INF_TRY(launch_pdl(kv->dtype == InfBF16 ? k_attn_chunk_combine<bf16> : k_attn_chunk_combine<float>, grid,
+		                   dim3(kAcCombineThreads), 0, st, b, p.R));
 	}
 	return Success;
 }

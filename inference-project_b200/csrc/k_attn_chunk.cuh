@@ -41,7 +41,7 @@ struct AttnChunkArgs {
 	int rows_min, rows_max;
 	int workers;
 	int min_run;                   // key tiles of a worker at least
-	float* part;                   // [2 * workers][R][hd + 2] partial O (unnormalised), max (log2 units), sum
+	float* part;                   // [2 * workers][hd + 2][R] partial O (unnormalised), max (log2 units), sum
 	int* jobs;                     // [workers][kAcJobInts]: the item that a worker begins and others end
 };
 
@@ -270,55 +270,65 @@ __device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w, const AcRu
 __host__ __device__ constexpr size_t ac_part_floats(int R, int hd) { return (size_t)R * (hd + 2); }
 
 // Joins the shares of every item that a cut divides: blockIdx.x is the worker that began it, blockIdx.y a
-// block of rows.  A partial holds O as [hd / 4][R] float4 when `columns`, else [R][hd], then the rows'
-// max and sum.
+// block of 32 rows.  A partial holds O as [hd / 4][R] float4, then the rows' max and sum.
 //   m = max_i m_i,  O = sum_i 2^(m_i - m) O_i,  l = sum_i 2^(m_i - m) l_i,  out = O / l
+// A lane owns a row, so that a warp's reads are whole lines; the eight warps share the head dims.
+constexpr int kAcCombineThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(256) k_attn_chunk_combine(const AttnChunkArgs a, int R, int columns)
+__global__ void __launch_bounds__(kAcCombineThreads) k_attn_chunk_combine(const AttnChunkArgs a, int R)
 {
 	pdl_wait();
 	pdl_trigger();
 	const int w0 = blockIdx.x;
 	const int* j = a.jobs + (size_t)w0 * kAcJobInts;
 	const int rows = j[kAcJobRows];
-	if (rows == 0) return;
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 32 + lane;
+	if (r >= rows) return;
 	const int last = j[kAcJobLast], hd4 = a.hd / 4;
 	const size_t pf = ac_part_floats(R, a.hd);
-	const float* first = a.part + (size_t)(2 * w0 + 1) * pf; // the beginner's share; the others' are slot 2 w
-	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-	for (int r = blockIdx.y * warps + warp; r < rows; r += gridDim.y * warps) {
-		auto part = [&](int w) { return w == w0 ? first : a.part + (size_t)(2 * w) * pf; };
-		float m = -INFINITY;
-		for (int w = w0 + lane; w <= last; w += kWarp) m = fmaxf(m, part(w)[(size_t)R * a.hd + r]);
-		m = warp_max(m);
-		float l = 0.0f;
-		for (int w = w0 + lane; w <= last; w += kWarp) {
-			const float* p = part(w) + (size_t)R * a.hd;
-			l += p[r] == -INFINITY ? 0.0f : exp2f(p[r] - m) * p[R + r];
-		}
-		l = warp_sum(l);
-		const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-		const int fr = j[kAcJobRow] + r;
-		T* out = reinterpret_cast<T*>(a.out) + (size_t)(j[kAcJobSeq] + fr / a.G) * a.out_stride +
-		         (size_t)(j[kAcJobHead] * a.G + fr % a.G) * a.hd;
-		for (int c = lane; c < hd4; c += kWarp) {
-			float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+	// the beginner's share is its second slot, the others' their first
+	auto part = [&](int w) { return a.part + (size_t)(2 * w + (w == w0 ? 1 : 0)) * pf; };
+	float m = -INFINITY;
 #pragma unroll 4
-			for (int w = w0; w <= last; ++w) {
-				const float* p = part(w);
-				const float mw = p[(size_t)R * a.hd + r];
-				const float f = mw == -INFINITY ? 0.0f : exp2f(mw - m);
-				const float4 v = reinterpret_cast<const float4*>(p)[columns ? (size_t)c * R + r : (size_t)r * hd4 + c];
-				if (f == 0.0f) continue; // a share without keys may hold anything
-				o.x = fmaf(f, v.x, o.x);
-				o.y = fmaf(f, v.y, o.y);
-				o.z = fmaf(f, v.z, o.z);
-				o.w = fmaf(f, v.w, o.w);
+	for (int w = w0; w <= last; ++w) m = fmaxf(m, part(w)[(size_t)R * a.hd + r]);
+	if (m == -INFINITY) m = 0.0f; // every share without keys: weights of 2^-inf = 0
+	float l = 0.0f;
+#pragma unroll 4
+	for (int w = w0; w <= last; ++w) {
+		const float* p = part(w) + (size_t)R * a.hd + r;
+		l = fmaf(exp2f(p[0] - m), p[R], l);
+	}
+	const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+	const int fr = j[kAcJobRow] + r;
+	T* out = reinterpret_cast<T*>(a.out) + (size_t)(j[kAcJobSeq] + fr / a.G) * a.out_stride +
+	         (size_t)(j[kAcJobHead] * a.G + fr % a.G) * a.hd;
+	constexpr int kWarps = kAcCombineThreads / kWarp, kCols = 4;
+	for (int c0 = warp * kCols; c0 < hd4; c0 += kWarps * kCols) {
+		float4 o[kCols];
+#pragma unroll
+		for (int c = 0; c < kCols; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+		for (int w = w0; w <= last; ++w) {
+			const float* p = part(w);
+			const float f = exp2f(p[(size_t)R * a.hd + r] - m);
+#pragma unroll
+			for (int c = 0; c < kCols; ++c) {
+				if (c0 + c >= hd4) continue;
+				const float4 v = reinterpret_cast<const float4*>(p)[(size_t)(c0 + c) * R + r];
+				o[c].x = fmaf(f, v.x, o[c].x);
+				o[c].y = fmaf(f, v.y, o[c].y);
+				o[c].z = fmaf(f, v.z, o[c].z);
+				o[c].w = fmaf(f, v.w, o[c].w);
 			}
-			Store<T>::put(out + 4 * c, o.x * inv);
-			Store<T>::put(out + 4 * c + 1, o.y * inv);
-			Store<T>::put(out + 4 * c + 2, o.z * inv);
-			Store<T>::put(out + 4 * c + 3, o.w * inv);
+		}
+#pragma unroll
+		for (int c = 0; c < kCols; ++c) {
+			if (c0 + c >= hd4) continue;
+			T* d = out + 4 * (c0 + c);
+			Store<T>::put(d, o[c].x * inv);
+			Store<T>::put(d + 1, o[c].y * inv);
+			Store<T>::put(d + 2, o[c].z * inv);
+			Store<T>::put(d + 3, o[c].w * inv);
 		}
 	}
 }
@@ -494,7 +504,7 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 #pragma unroll
 				for (int v = 0; v < VPL; ++v) {
 					const int c = lane + v * kWarp;
-					if (c < hd4) reinterpret_cast<float4*>(part)[(size_t)r * hd4 + c] = o[i][v];
+					if (c < hd4) reinterpret_cast<float4*>(part)[(size_t)c * kAfR + r] = o[i][v];
 				}
 				if (lane == 0) {
 					part[(size_t)kAfR * hd + r] = m[i];
