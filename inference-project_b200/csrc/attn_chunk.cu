@@ -97,11 +97,17 @@ Error_t launch_tc(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
 {
 	const u32 blk = (u32)a.blk, box = kCtKT / blk;
 	CUtensorMap k8, k1, v8, v1;
-	INF_TRY(tensor_map_kv(&k8, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
-	INF_TRY(tensor_map_kv(&k1, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
-	INF_TRY(tensor_map_kv(&v8, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
-	INF_TRY(tensor_map_kv(&v1, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
+	INF_TRY(tensor_map_kv_groups(&k8, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
+	INF_TRY(tensor_map_kv_groups(&k1, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
+	INF_TRY(tensor_map_kv_groups(&v8, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
+	INF_TRY(tensor_map_kv_groups(&v1, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
 	INF_TRY(allow_smem(k_attn_chunk_tc<HD>, 227 * 1024));
+	// the kernel's warpgroups trade registers within what it was launched with
+	static const int regs = [] {
+		cudaFuncAttributes f;
+		return cudaFuncGetAttributes(&f, k_attn_chunk_tc<HD>) == cudaSuccess ? f.numRegs : 0;
+	}();
+	if (regs < kCtRegsLaunch) return fail(ErrorUnsupported, "inf_attn_chunk: built with %d registers a thread", regs);
 	return launch_pdl(k_attn_chunk_tc<HD>, dim3((unsigned)p.workers), dim3(kCtThreads), p.smem, st, k8, k1, v8, v1, a);
 }
 
@@ -159,6 +165,7 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 	a.H = (int)A.n_heads;
 	a.KV = (int)kv->n_kv_heads;
 	a.G = a.H / a.KV;
+	a.group = ac_div(a.G);
 	a.hd = (int)kv->head_dim;
 	a.blk = (int)kv->kv_block;
 	a.n_slots = (int)kv->n_slots;

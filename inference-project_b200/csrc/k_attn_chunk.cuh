@@ -20,6 +20,22 @@ namespace inf {
 
 constexpr int kAcMaxSeqs = 4096;
 
+// n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and mul = floor(2^(31+s) / d) + 1 the error
+// of n * mul / 2^(31+s) stays below 1 / d (Granlund and Montgomery, PLDI 1994)
+struct AcDiv {
+	int d;
+	uint32_t mul;
+	int shift;
+	__device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+	__device__ __forceinline__ int mod(int n) const { return n - div(n) * d; }
+};
+inline AcDiv ac_div(int d)
+{
+	int s = 0;
+	while ((1ll << s) < d) ++s;
+	return {d, (uint32_t)((1ull << (31 + s)) / (uint64_t)d + 1), 31 + s};
+}
+
 struct AttnChunkArgs {
 	const void* q;
 	void* out;
@@ -32,6 +48,7 @@ struct AttnChunkArgs {
 	const int* seq_slot;           // null: sequence s is slot s
 	int n_seqs, n_tokens, max_new;
 	int H, KV, G, hd, blk;
+	AcDiv group;                   // by G
 	int n_slots, pages_per_seq, n_pages;
 	int window, n_sink;            // window 0: none
 	float scale;
@@ -86,7 +103,7 @@ template <int KT>
 __device__ __forceinline__ AcTiles ac_tiles(const AttnChunkArgs& a, const AcSeq& q, int r0, int r1)
 {
 	AcTiles t;
-	const int p0 = q.ctx - q.n + r0 / a.G, p1 = q.ctx - q.n + (r1 - 1) / a.G;
+	const int p0 = q.ctx - q.n + a.group.div(r0), p1 = q.ctx - q.n + a.group.div(r1 - 1);
 	t.hi = p1 + 1;
 	t.lo = a.window ? max(0, p0 - a.window + 1) : 0;
 	const int sinks = min(min(a.n_sink, t.lo), max(t.hi, 0)); // sinks below the window
@@ -300,8 +317,8 @@ __global__ void __launch_bounds__(kAcCombineThreads) k_attn_chunk_combine(const 
 	}
 	const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 	const int fr = j[kAcJobRow] + r;
-	T* out = reinterpret_cast<T*>(a.out) + (size_t)(j[kAcJobSeq] + fr / a.G) * a.out_stride +
-	         (size_t)(j[kAcJobHead] * a.G + fr % a.G) * a.hd;
+	T* out = reinterpret_cast<T*>(a.out) + (size_t)(j[kAcJobSeq] + a.group.div(fr)) * a.out_stride +
+	         (size_t)(j[kAcJobHead] * a.G + a.group.mod(fr)) * a.hd;
 	constexpr int kWarps = kAcCombineThreads / kWarp, kCols = 4;
 	for (int c0 = warp * kCols; c0 < hd4; c0 += kWarps * kCols) {
 		float4 o[kCols];
@@ -380,8 +397,8 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 			uint4 v = make_uint4(0, 0, 0, 0);
 			if (r < rows) {
 				const int fr = r0 + r;
-				v = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (size_t)(run.q.row0 + fr / a.G) * a.q_stride +
-				                                   (size_t)(run.h * a.G + fr % a.G) * hd)[c];
+				v = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (size_t)(run.q.row0 + a.group.div(fr)) * a.q_stride +
+				                                   (size_t)(run.h * a.G + a.group.mod(fr)) * hd)[c];
 			}
 			unpack_unit(v, f, (const T*)nullptr);
 #pragma unroll
@@ -395,7 +412,7 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 			m[i] = -INFINITY;
 			l[i] = 0.0f;
 			const int r = warp * kAfRows + i;
-			pos[i] = r < rows ? base_pos + (r0 + r) / a.G : -1;
+			pos[i] = r < rows ? base_pos + a.group.div(r0 + r) : -1;
 #pragma unroll
 			for (int v = 0; v < VPL; ++v) o[i][v] = make_float4(0.f, 0.f, 0.f, 0.f);
 		}
@@ -490,7 +507,7 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 			if (whole) {
 				const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
 				const int fr = r0 + r;
-				T* out = reinterpret_cast<T*>(a.out) + (size_t)(run.q.row0 + fr / a.G) * a.out_stride + (size_t)(run.h * a.G + fr % a.G) * hd;
+				T* out = reinterpret_cast<T*>(a.out) + (size_t)(run.q.row0 + a.group.div(fr)) * a.out_stride + (size_t)(run.h * a.G + a.group.mod(fr)) * hd;
 #pragma unroll
 				for (int v = 0; v < VPL; ++v) {
 					const int c = lane + v * kWarp;

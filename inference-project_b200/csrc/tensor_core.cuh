@@ -130,6 +130,38 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
 	    : "memory");
 }
 
+// mbar_wait timed by the SM's cycle counter: reading %globaltimer takes about a thousand cycles, which a
+// pipeline that waits at every tile pays each time a phase is not complete at once.  4e9 cycles are 2 s at
+// 2 GHz.
+constexpr long long kWaitLimitCycles = 4000000000ll;
+__device__ __forceinline__ bool mbar_wait_cycles(uint64_t* bar, uint32_t parity, volatile int* abort, int* err)
+{
+	if (mbar_try_wait(bar, parity)) return true;
+	const long long t0 = clock64();
+	for (uint32_t it = 1;; ++it) {
+		if (mbar_try_wait(bar, parity)) return true;
+		if ((it & 63u) == 0) {
+			if (*abort) return false;
+			if (clock64() - t0 > kWaitLimitCycles) {
+				*abort = 1;
+				report_err(err, kDevTimeout);
+				return false;
+			}
+		}
+	}
+}
+
+// 5-D tiled TMA load
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4, uint64_t* bar,
+                                            uint64_t policy)
+{
+	asm volatile(
+	    "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+	    " [%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(smem_u32(dst)),
+	    "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar)), "l"(policy)
+	    : "memory");
+}
+
 // byte offset of 16-byte chunk c (0..7) of row r inside a SWIZZLE_128B block of 128-byte rows
 __device__ __forceinline__ uint32_t sw128_off(int r, int c)
 {
