@@ -64,15 +64,16 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 		return Success;
 	};
 	const u32 blk = kv->kv_block;
-	if (kv->dtype == InfBF16 && (kv->head_dim == 64 || kv->head_dim == 128) && (blk == 16 || blk == 32 || blk == 64 || blk == 128)) {
+	const u32 G = n_heads / kv->n_kv_heads;
+	if (kv->dtype == InfBF16 && G <= kCtRows && (kv->head_dim == 64 || kv->head_dim == 128) && (blk == 16 || blk == 32 || blk == 64 || blk == 128)) {
 		ChunkPass t = {};
 		t.kind = ChunkPass::TC;
 		t.rows_max = 0x7FFFFFFF;
-		t.R = kCtR;
+		t.R = (int)(2 * (kCtRows / G) * G); // whole tokens in each half
 		t.min_run = 2;
 		t.smem = ct_layout((int)kv->head_dim, (int)n_seqs).total;
 		t.workers = sms;
-		return add(t, units_max(kv, n_heads, n_tokens, n_seqs, kCtR, kCtKT));
+		return add(t, units_max(kv, n_heads, n_tokens, n_seqs, (u32)t.R, kCtKT));
 	}
 	ChunkPass f = {};
 	f.kind = ChunkPass::F32;
@@ -96,7 +97,8 @@ template <int HD>
 Error_t launch_tc(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
 {
 	const u32 blk = (u32)a.blk, box = kCtKT / blk;
-	CUtensorMap k8, k1, v8, v1;
+	CUtensorMap q, k8, k1, v8, v1;
+	INF_TRY(tensor_map_q(&q, a.q, (u32)a.n_tokens, (u32)a.H, HD, a.q_stride, (u32)a.G, (u32)(kCtRows / a.G)));
 	INF_TRY(tensor_map_kv_groups(&k8, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
 	INF_TRY(tensor_map_kv_groups(&k1, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
 	INF_TRY(tensor_map_kv_groups(&v8, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
@@ -108,7 +110,7 @@ Error_t launch_tc(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
 		return cudaFuncGetAttributes(&f, k_attn_chunk_tc<HD>) == cudaSuccess ? f.numRegs : 0;
 	}();
 	if (regs < kCtRegsLaunch) return fail(ErrorUnsupported, "inf_attn_chunk: built with %d registers a thread", regs);
-	return launch_pdl(k_attn_chunk_tc<HD>, dim3((unsigned)p.workers), dim3(kCtThreads), p.smem, st, k8, k1, v8, v1, a);
+	return launch_pdl(k_attn_chunk_tc<HD>, dim3((unsigned)p.workers), dim3(kCtThreads), p.smem, st, q, k8, k1, v8, v1, a);
 }
 
 } // namespace
@@ -132,7 +134,7 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 	INF_TRY(chunk_plan(kv, A.n_heads, A.n_tokens, A.n_seqs, &P));
 	const u64 es = kv->dtype == InfBF16 ? 2 : 4, row = (u64)A.n_heads * kv->head_dim;
 	const u64 qs = A.q_stride ? A.q_stride : row, os = A.out_stride ? A.out_stride : row;
-	if (qs < row || os < row || qs > (1ull << 40) || os > (1ull << 40) || (qs * es) % 16 || (os * es) % 16)
+	if (qs < row || os < row || qs > (1ull << 38) || os > (1ull << 38) || (qs * es) % 16 || (os * es) % 16)
 		return fail(ErrorInvalidValue, "%s: row strides", who);
 	if (!(A.scale >= 0.0f) || !std::isfinite(A.scale)) return fail(ErrorInvalidValue, "%s: scale %g", who, A.scale);
 	if (A.n_seqs == 0 || A.n_tokens == 0) return Success;
@@ -181,6 +183,7 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 		AttnChunkArgs b = a;
 		b.rows_min = p.rows_min;
 		b.rows_max = p.rows_max;
+		b.R = p.R;
 		b.workers = p.workers;
 		b.min_run = p.min_run;
 		b.part = (float*)((uint8_t*)A.scratch + p.part_off);
@@ -197,7 +200,7 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 		const AttnChunkArgs b = pass_args(p);
 		const dim3 grid((unsigned)p.workers, (unsigned)((p.R + 31) / 32));
 		INF_TRY(launch_pdl(kv->dtype == InfBF16 ? k_attn_chunk_combine<bf16> : k_attn_chunk_combine<float>, grid,
-		                   dim3(kAcCombineThreads), 0, st, b, p.R));
+		                   dim3(kAcCombineThreads), 0, st, b));
 	}
 	return Success;
 }

@@ -215,6 +215,21 @@ Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv,
 	return Success;
 }
 
+Error_t tensor_map_q(CUtensorMap* m, const void* base, u32 tokens, u32 heads, u32 hd, u64 stride, u32 box_heads, u32 box_tokens)
+{
+	PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+	INF_TRY(tensor_map_encoder(&encode));
+	const cuuint64_t dims[3] = {hd, heads, tokens};
+	const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2};
+	const cuuint32_t box[3] = {64, box_heads, box_tokens};
+	const cuuint32_t estr[3] = {1, 1, 1};
+	const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+	                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+	                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+	if (r != CUDA_SUCCESS) return fail(ErrorCuda, "cuTensorMapEncodeTiled (queries) failed (%d)", (int)r);
+	return Success;
+}
+
 Error_t tensor_map_kv_groups(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages)
 {
 	PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;

@@ -3,7 +3,7 @@
 // every type and head size.
 //
 // An item is (sequence, KV head, row tile): the rows of a sequence and KV head are its new tokens times
-// the G query heads of the group, row r = token * G + head, R of them to a tile, so K and V are read
+// the G query heads of the group, row r = token * G + head, R of them to an item, so K and V are read
 // once per tile for the whole group.  The keys an item sees come in key tiles of KT positions: those of
 // the sinks, then those from the window's start to the last row's position; their number is the item's
 // cost.  All costs laid end to end (sequence, head, tile) are cut into equal runs, one per worker: a
@@ -56,6 +56,7 @@ struct AttnChunkArgs {
 	// division of the work: sequences with more than rows_min and at most rows_max rows per KV head
 	// belong to this launch
 	int rows_min, rows_max;
+	int R;                         // rows of an item
 	int workers;
 	int min_run;                   // key tiles of a worker at least
 	float* part;                   // [2 * workers][hd + 2][R] partial O (unnormalised), max (log2 units), sum
@@ -122,17 +123,18 @@ __device__ __forceinline__ bool ac_sees(const AttnChunkArgs& a, int p, int k)
 	return k <= p && (a.window == 0 || k > p - a.window || k < a.n_sink);
 }
 
-template <int R, int KT>
+template <int KT>
 __device__ __forceinline__ int ac_tile_cost(const AttnChunkArgs& a, const AcSeq& q, int tile)
 {
-	return ac_tiles<KT>(a, q, tile * R, min((tile + 1) * R, q.n * a.G)).cost;
+	return ac_tiles<KT>(a, q, tile * a.R, min((tile + 1) * a.R, q.n * a.G)).cost;
 }
 
 // pre[s] = cost of the sequences before s over all heads, pre[n_seqs] = the total.  Every thread of the
 // CTA calls it (blockDim a multiple of 32, at most 1024); ends with a barrier.
-template <int R, int KT>
+template <int KT>
 __device__ __forceinline__ void ac_prefix(const AttnChunkArgs& a, uint32_t* pre)
 {
+	const int R = a.R;
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 	const bool report = blockIdx.x == 0;
 	// a lane per sequence when tiles are few; a warp per sequence, its lanes over the tiles, otherwise
@@ -140,15 +142,15 @@ __device__ __forceinline__ void ac_prefix(const AttnChunkArgs& a, uint32_t* pre)
 		for (int s = threadIdx.x; s < a.n_seqs; s += blockDim.x) {
 			const AcSeq q = ac_seq(a, s, report);
 			uint32_t c = 0;
-			for (int t = 0; t * R < q.n * a.G; ++t) c += ac_tile_cost<R, KT>(a, q, t);
+			for (int t = 0; t * R < q.n * a.G; ++t) c += ac_tile_cost<KT>(a, q, t);
 			pre[s + 1] = c * (uint32_t)a.KV;
 		}
 	} else {
 		for (int s = warp; s < a.n_seqs; s += warps) {
 			const AcSeq q = ac_seq(a, s, report && lane == 0);
-			const int tiles = (q.n * a.G + R - 1) / R;
+			const int rows = q.n * a.G;
 			uint32_t c = 0;
-			for (int t = lane; t < tiles; t += kWarp) c += ac_tile_cost<R, KT>(a, q, t);
+			for (int t = lane; t * R < rows; t += kWarp) c += ac_tile_cost<KT>(a, q, t);
 #pragma unroll
 			for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
 			if (lane == 0) pre[s + 1] = c * (uint32_t)a.KV;
@@ -174,7 +176,7 @@ __device__ __forceinline__ void ac_prefix(const AttnChunkArgs& a, uint32_t* pre)
 }
 
 // A worker's run of the laid-out costs, walked item by item (every lane of the warp holds the same).
-template <int R, int KT>
+template <int KT>
 struct AcRun {
 	uint32_t at, end, run; // position and end of the run, length of every run
 	int s, h, tile, tiles;
@@ -187,16 +189,16 @@ struct AcRun {
 	__device__ __forceinline__ int from() const { return (int)(at - item); }
 	__device__ __forceinline__ int to() const { return (int)(min(end, item + (uint32_t)t.cost) - item); }
 	__device__ __forceinline__ bool whole() const { return from() == 0 && to() == t.cost; }
-	__device__ __forceinline__ int rows() const { return min(R, q.n * g_ - tile * R); }
+	__device__ __forceinline__ int rows() const { return min(r_, rows_ - tile * r_); }
 	// slot of the partial: a worker ends at most one item that began before it and begins at most one
 	// that ends after it
 	__device__ __forceinline__ int slot(int worker) const { return 2 * worker + (from() == 0 ? 1 : 0); }
 	__device__ __forceinline__ int last_worker() const { return (int)((item + (uint32_t)t.cost - 1) / run); }
-	int g_;
+	int r_, rows_; // rows of an item, rows of the sequence
 
 	__device__ __forceinline__ void tile_of(const AttnChunkArgs& a)
 	{
-		t = ac_tiles<KT>(a, q, tile * R, min((tile + 1) * R, q.n * a.G));
+		t = ac_tiles<KT>(a, q, tile * r_, min((tile + 1) * r_, rows_));
 	}
 
 	// by a whole warp
@@ -208,7 +210,7 @@ struct AcRun {
 		const uint64_t b = (uint64_t)run * (uint32_t)worker;
 		at = b < total ? (uint32_t)b : total;
 		end = (uint32_t)min(b + run, (uint64_t)total);
-		g_ = a.G;
+		r_ = a.R;
 		if (done()) return;
 		int l = 0, r = a.n_seqs; // the last s with pre[s] <= at
 		while (r - l > 1) {
@@ -218,7 +220,8 @@ struct AcRun {
 		}
 		s = l;
 		q = ac_seq(a, s, false);
-		tiles = (q.n * a.G + R - 1) / R;
+		rows_ = q.n * a.G;
+		tiles = (rows_ + r_ - 1) / r_;
 		const uint32_t per_head = (pre[s + 1] - pre[s]) / (uint32_t)a.KV;
 		const uint32_t in = at - pre[s];
 		h = (int)(in / per_head);
@@ -227,7 +230,7 @@ struct AcRun {
 		// the tile that holds `left`: 32 tiles at a time
 		for (tile = 0;; tile += kWarp) {
 			const int my = tile + lane;
-			const uint32_t c = my < tiles ? (uint32_t)ac_tile_cost<R, KT>(a, q, my) : 0u;
+			const uint32_t c = my < tiles ? (uint32_t)ac_tile_cost<KT>(a, q, my) : 0u;
 			uint32_t x = c;
 #pragma unroll
 			for (int o = 1; o < 32; o <<= 1) {
@@ -260,7 +263,8 @@ struct AcRun {
 				do ++s;
 				while (pre[s + 1] == pre[s]);
 				q = ac_seq(a, s, false);
-				tiles = (q.n * a.G + R - 1) / R;
+				rows_ = q.n * a.G;
+				tiles = (rows_ + r_ - 1) / r_;
 			}
 		}
 		tile_of(a);
@@ -268,8 +272,8 @@ struct AcRun {
 };
 
 // The record of an item that worker `w` begins and does not end (one lane calls it), or of none.
-template <int R, int KT>
-__device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w, const AcRun<R, KT>* run)
+template <int KT>
+__device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w, const AcRun<KT>* run)
 {
 	int* j = a.jobs + (size_t)w * kAcJobInts;
 	if (!run) {
@@ -278,7 +282,7 @@ __device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w, const AcRu
 	}
 	j[kAcJobSeq] = run->q.row0;
 	j[kAcJobHead] = run->h;
-	j[kAcJobRow] = run->tile * R;
+	j[kAcJobRow] = run->tile * a.R;
 	j[kAcJobRows] = run->rows();
 	j[kAcJobLast] = run->last_worker();
 }
@@ -292,8 +296,9 @@ __host__ __device__ constexpr size_t ac_part_floats(int R, int hd) { return (siz
 // A lane owns a row, so that a warp's reads are whole lines; the eight warps share the head dims.
 constexpr int kAcCombineThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(kAcCombineThreads) k_attn_chunk_combine(const AttnChunkArgs a, int R)
+__global__ void __launch_bounds__(kAcCombineThreads) k_attn_chunk_combine(const AttnChunkArgs a)
 {
+	const int R = a.R;
 	pdl_wait();
 	pdl_trigger();
 	const int w0 = blockIdx.x;
@@ -380,10 +385,10 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 	float* p_s = kv_s + kAfKT * ld;       // [16][32]
 	uint32_t* pre = reinterpret_cast<uint32_t*>(p_s + kAfR * kAfKT);
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, worker = blockIdx.x;
-	ac_prefix<kAfR, kAfKT>(a, pre);
-	AcRun<kAfR, kAfKT> run;
+	ac_prefix<kAfKT>(a, pre);
+	AcRun<kAfKT> run;
 	run.begin(a, pre, worker);
-	if (threadIdx.x == 0) ac_job<kAfR, kAfKT>(a, worker, nullptr);
+	if (threadIdx.x == 0) ac_job<kAfKT>(a, worker, nullptr);
 	const float sl2 = a.scale * 1.4426950408889634f;
 	constexpr int V = Store<T>::kVec;
 	for (; !run.done(); run.next(a, pre)) {
@@ -529,7 +534,7 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 				}
 			}
 		}
-		if (!whole && run.from() == 0 && threadIdx.x == 0) ac_job<kAfR, kAfKT>(a, worker, &run);
+		if (!whole && run.from() == 0 && threadIdx.x == 0) ac_job<kAfKT>(a, worker, &run);
 	}
 }
 

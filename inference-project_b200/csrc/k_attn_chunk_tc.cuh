@@ -1,22 +1,23 @@
 // Chunk attention on the 5th-generation tensor cores (bf16, head_dim 64 or 128, pages of 16 .. 128).
 //
-// A CTA is a worker of k_attn_chunk.cuh with items of 256 rows (256 / G tokens times the G heads of a KV
-// group) and key tiles of 128 positions.  The rows are two subtiles of 128, each with its own softmax
-// warpgroup, so that one subtile's exponentials run while the tensor cores work on the other's products:
-//   warps 0-3, 4-7  a thread per row of subtile 0, 1: Q into shared memory (SWIZZLE_128B by hand), then per
-//                   key tile S from tensor memory, mask, running max and sum, P = 2^(s scale - m) as bf16
-//                   back into the same tensor-memory columns, in two halves; O / sum at the end
+// A CTA is a worker of k_attn_chunk.cuh with items of up to 256 rows (2 floor(128 / G) tokens times the G
+// heads of a KV group) and key tiles of 128 positions.  The rows are two subtiles of up to 128, each with its
+// own warpgroup, so that one subtile's exponentials run while the tensor cores work on the other's products:
+//   warps 0-3, 4-7  a thread per row of subtile 0, 1: per key tile S from tensor memory into registers, mask,
+//                   running max, P = 2^(s scale - m) as bf16 back into the same tensor-memory columns in two
+//                   halves, then the row's sum (off the path to the next product); O / sum at the end
 //   warps 8, 10     TMA producers of K and of V tiles into one ring (no multicast): a 5-D box per page, [8-row
 //                   group][64 head dims][8 x 128 bytes], or one for the whole tile where the page ids are
-//                   consecutive.  A box costs its producer about 90 cycles of issue, so that a box per page and 64
-//                   head dims from one warp (32 a key tile) had paced the kernel at 4200 cycles a key tile.
-//   warp 9          one thread issues S = Q.K^T (shared memory x shared memory) and O += P.V (P from
-//                   tensor memory, V MN-major from shared memory)
+//                   consecutive
+//   warp 9          issues S = Q.K^T (shared memory x shared memory) and O += P.V (P from tensor memory, V
+//                   MN-major from shared memory)
+//   warp 11         TMA producer of Q: a box of floor(128 / G) tokens x G heads per subtile and 64 head dims
 // Tensor memory (512 columns): S0 | S1 | O0 | O1, P over the first half of its S.  The issue order
 //   S0(0) S1(0) | PV0(j) S0(j+1) PV1(j) S1(j+1) | ...
-// keeps S(j+1) behind the P(j) that it overwrites, and a completed S(j+1) implies a completed PV(j): O may
-// then be rescaled without another wait.  That happens only when a row's max grows by more than 2^8
-// (bf16 and fp32 hold the larger weights as well, and O / sum is unchanged).
+// keeps S(j+1) behind the P(j) that it overwrites, keeps the subtiles half a period apart (when each
+// warpgroup issued its own products both waited and both computed at the same time), and makes a completed
+// S(j+1) imply a completed PV(j): O may then be rescaled without another wait.  That happens only when a
+// row's max grows by more than 2^8 (bf16 and fp32 hold the larger weights as well, and O / sum is unchanged).
 // Rounding: S, O, max and sum are fp32; P is rounded to bf16 for the second product, the sum adds the
 // unrounded weights (their rounding errors are independent and average out).
 // Positions that no row of the item sees are not loaded page by page; where they share a page with seen
@@ -31,23 +32,23 @@
 
 namespace inf {
 
-constexpr int kCtR = 256;
+constexpr int kCtRows = 128; // rows of a subtile at most: floor(128 / G) tokens times G heads
 constexpr int kCtKT = 128;
-constexpr int kCtThreads = 384; // 3 warpgroups: softmax, softmax, (TMA, MMA, TMA, idle)
-// Registers: 168 a thread at launch; the softmax warpgroups, which hold a row of 128 scores, take the third
+constexpr int kCtThreads = 384; // 3 warpgroups: subtile 0, subtile 1, copies and products
+// Registers: 168 a thread at launch; the softmax warpgroups, which hold a row of 128 scores, take of the third
 // one's share: 2 x 208 + 88 = 3 x 168.
 constexpr int kCtRegsLaunch = 168, kCtRegsSoftmax = 208, kCtRegsRest = 88;
 static_assert(2 * kCtRegsSoftmax + kCtRegsRest <= 3 * kCtRegsLaunch, "register split");
 constexpr int kCtMaxStages = 12;
 constexpr uint32_t kCtAtom = 128 * 64 * 2; // one [128 x 64] bf16 SWIZZLE_128B block: 16 KB
 constexpr float kCtRescaleLog2 = 8.0f;
-constexpr int kCtPolyOf8 = 2; // of 8 pairs of weights, those whose 2^x runs on the FMA pipes
 
 enum CtBar : int {
-	kCtFull = 0,                          // [stages] TMA -> MMA (and the softmax warps, for V)
-	kCtEmpty = kCtMaxStages,              // [stages] MMA done with the tile
-	kCtQ = 2 * kCtMaxStages,              // [2] Q of the subtile staged (4 warps arrive)
-	kCtS = kCtQ + 2,                      // [2] S ready
+	kCtFull = 0,                          // [stages] tile in the ring
+	kCtEmpty = kCtMaxStages,              // [stages] both subtiles' products done with it
+	kCtQ = 2 * kCtMaxStages,              // [2] Q of the subtile loaded
+	kCtQFree = kCtQ + 2,                  // [2] the item's last S done with it
+	kCtS = kCtQFree + 2,                  // [2] S ready
 	kCtP = kCtS + 2,                      // [2][2] P's halves written (4 warps arrive)
 	kCtO = kCtP + 4,                      // [2] the item's last product done
 	kCtDrain = kCtO + 2,
@@ -108,29 +109,6 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b)
 	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
 	return r;
 }
-// 2^x of two values on the FMA pipes, for the share of the weights that would otherwise queue for the
-// special-function unit: x = n + f with n the nearest integer (the low bits of x + 1.5 * 2^23), 2^f by the
-// minimax polynomial of degree 3 on [-1/2, 1/2] (Remez exchange on the relative error: 7.5e-5 = 2^-13.7,
-// against the 2^-9 of the bf16 rounding that follows), n added to the exponent.  x below -126 gives
-// about 1e-38 instead of less.
-__device__ __forceinline__ void ex2_poly2(uint64_t x2, float& p0, float& p1)
-{
-	float x0, x1;
-	f2_split(x2, x0, x1);
-	x2 = f2(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
-	const uint64_t t = f2_add(x2, f2(12582912.0f, 12582912.0f));
-	const uint64_t n = f2_add(t, f2(-12582912.0f, -12582912.0f));
-	const uint64_t f = f2_fma(n, f2(-1.0f, -1.0f), x2);
-	uint64_t p = f2_fma(f, f2(0.0551716685f, 0.0551716685f), f2(0.2426111251f, 0.2426111251f));
-	p = f2_fma(p, f, f2(0.6932609677f, 0.6932609677f));
-	p = f2_fma(p, f, f2(0.9999280572f, 0.9999280572f));
-	float t0, t1;
-	f2_split(t, t0, t1);
-	f2_split(p, p0, p1);
-	p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-	p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
 __device__ __forceinline__ void tmem_st_16regs(uint32_t taddr, const uint32_t (&r)[16])
 {
 	asm volatile(
@@ -160,6 +138,49 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xF
 // the n lowest bits (none for n <= 0, all from 32 on)
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
 
+// 32 columns without the wait; the registers hold the values only behind tmem_ld_wait, which ties them to it
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, float (&v)[32])
+{
+	asm volatile(
+	    "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+	    "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+	    "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+	    : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+	      "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]),
+	      "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]),
+	      "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+	    : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait(float (&v)[32])
+{
+	asm volatile("tcgen05.wait::ld.sync.aligned;"
+	             : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+	               "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+	               "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+	               "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29])
+	             :
+	             : "memory");
+	asm volatile("" : "+f"(v[30]), "+f"(v[31]));
+}
+
+// 16 columns of O times f (a row each lane), in few registers: it runs while a row of scores is held
+__device__ __forceinline__ void tmem_scale_16(uint32_t taddr, float f)
+{
+	float v[16];
+	asm volatile(
+	    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+	    "tcgen05.wait::ld.sync.aligned;"
+	    : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+	      "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+	    : "r"(taddr)
+	    : "memory");
+	uint32_t w[16];
+#pragma unroll
+	for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i] * f);
+	tmem_st_16regs(taddr, w);
+	asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
 // position in the ring: stage and the parity of its use
 struct CtRing {
 	int stage = 0;
@@ -181,7 +202,7 @@ struct CtRing {
 
 template <int HD>
 __global__ void __launch_bounds__(kCtThreads, 1)
-    k_attn_chunk_tc(const __grid_constant__ CUtensorMap tm_k8, const __grid_constant__ CUtensorMap tm_k1,
+    k_attn_chunk_tc(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k8, const __grid_constant__ CUtensorMap tm_k1,
                     const __grid_constant__ CUtensorMap tm_v8, const __grid_constant__ CUtensorMap tm_v1, const AttnChunkArgs a)
 {
 	constexpr int kHalves = HD / 64;
@@ -201,8 +222,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 
 	if (threadIdx.x == 0) {
 		for (int i = 0; i < kCtBars; ++i) {
-			const bool warps = (i >= kCtQ && i < kCtS) || (i >= kCtP && i < kCtO); // the four warps of a warpgroup arrive
-			mbar_init(&bars[i], warps ? 4 : 1);
+			mbar_init(&bars[i], i >= kCtP && i < kCtO ? 4 : 1);
 		}
 		*abort_flag = 0;
 		mbar_fence_init();
@@ -214,10 +234,10 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 	pdl_wait();
 	pdl_trigger();
 	tc_fence_before();
-	ac_prefix<kCtR, kCtKT>(a, pre); // ends with a barrier
+	ac_prefix<kCtKT>(a, pre); // ends with a barrier
 	tc_fence_after();
 	const uint32_t tmem = *tmem_slot;
-	AcRun<kCtR, kCtKT> run;
+	AcRun<kCtKT> run;
 	run.begin(a, pre, worker);
 
 	if (warp >= 8) {
@@ -257,7 +277,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 				const bool one_box = mask == (1u << pages) - 1u && __all_sync(0xFFFFFFFFu, lane >= pages || page == page0 + lane);
 				const uint32_t bytes = (uint32_t)__popc(mask) * (uint32_t)blk * HD * 2;
 				if (entry >= (uint32_t)stages) {
-					const bool w = mbar_wait_cycles(&bars[kCtEmpty + r.stage], r.phase ^ 1u, abort_flag, a.status);
+					const bool w = mbar_wait_cycles<64>(&bars[kCtEmpty + r.stage], r.phase ^ 1u, abort_flag, a.status);
 					ok = __all_sync(0xFFFFFFFFu, w);
 					if (!ok) break;
 				}
@@ -296,7 +316,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 			}
 		}
 	} else if (warp == 9) {
-		// ---------------- MMA issuer: the warp runs the pipeline converged, one elected lane issues
+		// ---------------- product issuer: the warp runs the pipeline converged, one elected lane issues
 		constexpr uint32_t idesc_s = umma_idesc_bf16(128, kCtKT);
 		constexpr uint32_t idesc_o = umma_idesc_bf16(128, HD) | (1u << 16); // B (V) MN-major
 		const uint32_t qa = smem_u32(q_s), ra = smem_u32(ring_s), tm = uniform(tmem);
@@ -306,105 +326,143 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 			const bool w = mbar_wait_cycles(&bars[bar], par, abort_flag, a.status);
 			return (bool)__all_sync(0xFFFFFFFFu, w);
 		};
-		auto commit = [&](int bar) {
-			if (elect_one()) umma_commit(&bars[bar]);
-			__syncwarp();
-		};
-		auto issue_s = [&](int sub, uint32_t stage) {
+		auto mma_s = [&](int sub, uint32_t stage) { // by the elected lane
 			const uint64_t da = umma_desc_sw128(qa + (uint32_t)sub * kTile);
 			const uint64_t db = umma_desc_sw128_lbo(ra + stage * kTile, 16, kGroup);
-			if (elect_one()) {
 #pragma unroll
-				for (int k = 0; k < HD / 16; ++k)
-					umma_bf16(tm + (uint32_t)sub * kCtKT, da + (uint32_t)((k >> 2) * (kCtAtom / 16) + (k & 3) * 2),
-					          db + (uint32_t)((k >> 2) * 64 + (k & 3) * 2), idesc_s, k > 0 ? 1u : 0u);
-				umma_commit(&bars[kCtS + sub]);
-			}
-			__syncwarp();
+			for (int k = 0; k < HD / 16; ++k)
+				umma_bf16(tm + (uint32_t)sub * kCtKT, da + (uint32_t)((k >> 2) * (kCtAtom / 16) + (k & 3) * 2),
+				          db + (uint32_t)((k >> 2) * 64 + (k & 3) * 2), idesc_s, k > 0 ? 1u : 0u);
+			umma_commit(&bars[kCtS + sub]);
 		};
-		auto issue_pv = [&](int sub, uint32_t stage, uint32_t acc) -> bool {
+		auto mma_pv = [&](int sub, uint32_t stage, int half, uint32_t acc) {
 			const uint64_t dv = umma_desc_sw128_lbo(ra + stage * kTile, 1024, kGroup);
 			const uint32_t pa = tm + (uint32_t)sub * kCtKT, od = tm + 2 * kCtKT + (uint32_t)(sub * HD);
 #pragma unroll
-			for (int half = 0; half < 2; ++half) {
-				if (!wait(kCtP + sub * 2 + half, p_par[sub])) return false;
-				tc_fence_after();
-				if (elect_one()) {
-#pragma unroll
-					for (int k = half * 4; k < half * 4 + 4; ++k)
-						umma_bf16_ts(od, pa + (uint32_t)k * 8, dv + (uint32_t)(k * 2 * kGroup / 16), idesc_o, k > 0 ? 1u : acc);
-				}
-				__syncwarp();
-			}
-			p_par[sub] ^= 1u;
-			return true;
+			for (int k = half * 4; k < half * 4 + 4; ++k)
+				umma_bf16_ts(od, pa + (uint32_t)k * 8, dv + (uint32_t)(k * 2 * kGroup / 16), idesc_o, k > 0 ? 1u : acc);
 		};
 		bool ok = true;
 		for (; ok && !run.done(); run.next(a, pre)) {
 			const int n = run.to() - run.from();
-			const bool two = run.rows() > 128;
-			// K of the first tile
-			ok = wait(kCtFull + r.stage, r.phase) && wait(kCtQ, q_par[0]);
-			if (!ok) break;
-			q_par[0] ^= 1u;
-			tc_fence_after();
+			const int subs = run.rows() > (a.R >> 1) ? 2 : 1;
+			// S of the first tile
 			uint32_t ks = uniform((uint32_t)r.stage);
-			issue_s(0, ks);
-			if (two) {
-				ok = wait(kCtQ + 1, q_par[1]);
+			ok = wait(kCtFull + (int)ks, r.phase);
+#pragma unroll
+			for (int sub = 0; sub < 2; ++sub) {
+				if (!ok || sub >= subs) break;
+				ok = wait(kCtQ + sub, q_par[sub]);
 				if (!ok) break;
-				q_par[1] ^= 1u;
+				q_par[sub] ^= 1u;
 				tc_fence_after();
-				issue_s(1, ks);
+				if (elect_one()) {
+					mma_s(sub, ks);
+					if (n == 1) umma_commit(&bars[kCtQFree + sub]);
+					if (sub == subs - 1) umma_commit(&bars[kCtEmpty + ks]);
+				}
+				__syncwarp();
 			}
-			commit(kCtEmpty + (int)ks);
+			if (!ok) break;
 			r.next(stages);
 			for (int j = 0; ok && j < n; ++j) {
+				// V of this tile and K of the next are waited for ahead of P, so that nothing but the issue
+				// stands between P's second half and the next S
 				const uint32_t vs = uniform((uint32_t)r.stage);
 				ok = wait(kCtFull + (int)vs, r.phase);
 				if (!ok) break;
 				r.next(stages);
-				ok = issue_pv(0, vs, j > 0 ? 1u : 0u);
-				if (!ok) break;
-				ks = uniform((uint32_t)r.stage);
-				if (j + 1 < n) {
+				const bool more = j + 1 < n, last_s = j + 2 == n;
+				if (more) {
+					ks = uniform((uint32_t)r.stage);
 					ok = wait(kCtFull + (int)ks, r.phase);
 					if (!ok) break;
-					tc_fence_after();
-					issue_s(0, ks);
-				} else {
-					commit(kCtO);
-				}
-				if (two) {
-					ok = issue_pv(1, vs, j > 0 ? 1u : 0u);
-					if (!ok) break;
-				}
-				commit(kCtEmpty + (int)vs);
-				if (j + 1 < n) {
-					if (two) issue_s(1, ks);
-					commit(kCtEmpty + (int)ks);
 					r.next(stages);
-				} else if (two) {
-					commit(kCtO + 1);
+				}
+				const uint32_t acc = j > 0 ? 1u : 0u;
+#pragma unroll
+				for (int sub = 0; sub < 2; ++sub) {
+					if (!ok || sub >= subs) break;
+					ok = wait(kCtP + sub * 2, p_par[sub]);
+					if (!ok) break;
+					tc_fence_after();
+					if (elect_one()) mma_pv(sub, vs, 0, acc);
+					__syncwarp();
+					ok = wait(kCtP + sub * 2 + 1, p_par[sub]);
+					if (!ok) break;
+					p_par[sub] ^= 1u;
+					tc_fence_after();
+					if (elect_one()) {
+						mma_pv(sub, vs, 1, 1u);
+						if (more) {
+							mma_s(sub, ks);
+							if (last_s) umma_commit(&bars[kCtQFree + sub]);
+						} else {
+							umma_commit(&bars[kCtO + sub]);
+						}
+						if (sub == subs - 1) {
+							umma_commit(&bars[kCtEmpty + vs]);
+							if (more) umma_commit(&bars[kCtEmpty + ks]);
+						}
+					}
+					__syncwarp();
 				}
 			}
 		}
 		// every product is done before tensor memory is freed, whatever ended the loop
-		commit(kCtDrain);
+		if (elect_one()) umma_commit(&bars[kCtDrain]);
+		__syncwarp();
 		const long long t0 = clock64();
 		while (!mbar_try_wait(&bars[kCtDrain], 0))
 			if (clock64() - t0 > kWaitLimitCycles) break;
 		__syncwarp();
+	} else {
+		// ---------------- TMA producer of Q: both subtiles of the next item while the last one finishes
+		const uint32_t bytes = (uint32_t)(a.R >> 1) * HD * 2;
+		const int toks = a.group.div(a.R >> 1); // tokens of a subtile
+		const uint64_t pol = policy_evict_first();
+		uint32_t uses[2] = {0, 0};
+		bool ok = true;
+		for (; ok && !run.done(); run.next(a, pre)) {
+			const int subs = run.rows() > (a.R >> 1) ? 2 : 1;
+			const int head = (int)uniform((uint32_t)(run.h * a.G)), tok = (int)uniform((uint32_t)(run.q.row0 + run.tile * 2 * toks));
+#pragma unroll
+			for (int sub = 0; sub < 2; ++sub) {
+				if (!ok || sub >= subs) break;
+				if (uses[sub] > 0) {
+					const bool w = mbar_wait_cycles<500>(&bars[kCtQFree + sub], (uses[sub] - 1) & 1u, abort_flag, a.status);
+					ok = __all_sync(0xFFFFFFFFu, w);
+					if (!ok) break;
+				}
+				if (elect_one()) {
+					mbar_arrive_expect_tx(&bars[kCtQ + sub], bytes);
+#pragma unroll
+					for (int h = 0; h < kHalves; ++h)
+						tma_load_3d(q_s + (uint32_t)sub * kTile + h * kCtAtom, &tm_q, h * 64, head, tok + sub * toks, &bars[kCtQ + sub], pol);
+				}
+				__syncwarp();
+				++uses[sub];
+			}
+		}
+		if (!ok) {
+			for (int sub = 0; sub < 2; ++sub) { // copies in flight
+				if (uses[sub] == 0) continue;
+				const long long t0 = clock64();
+				while (!mbar_try_wait(&bars[kCtQ + sub], (uses[sub] - 1) & 1u))
+					if (clock64() - t0 > kWaitLimitCycles) break;
+			}
+		}
 	}
 	} else {
 		asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kCtRegsSoftmax));
 		// ---------------- softmax: subtile `sub`, a thread per row
 		const int sub = warp >> 2, quarter = warp & 3;
-		const int r = quarter * 32 + lane;
+		const int r = quarter * 32 + lane, half_rows = a.R >> 1;
 		const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
 		const uint32_t ts = tmem + (uint32_t)sub * kCtKT + lanes, to = tmem + 2 * kCtKT + (uint32_t)(sub * HD) + lanes;
-		uint8_t* qd = q_s + (size_t)sub * kTile;
 		const float sl2 = a.scale * 1.4426950408889634f; // scores in log2 units
+		const uint64_t sl2x2 = f2(sl2, sl2);
+		const int n_sink = a.n_sink;
 		CtRing ring;
 		uint32_t s_par = 0, o_par = 0;
 		bool ok = true;
@@ -413,38 +471,21 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 			const bool w = mbar_wait_cycles(&bars[bar], par, abort_flag, a.status);
 			return (bool)__all_sync(0xFFFFFFFFu, w);
 		};
-		if (warp == 0 && lane == 0) ac_job<kCtR, kCtKT>(a, worker, nullptr);
+		if (warp == 0 && lane == 0) ac_job<kCtKT>(a, worker, nullptr);
 		for (; ok && !run.done(); run.next(a, pre)) {
 			const int from = run.from(), to_tile = run.to();
-			const int valid = min(128, run.rows() - sub * 128); // rows of this subtile
-			if (warp == 0 && lane == 0 && from == 0 && !run.whole()) ac_job<kCtR, kCtKT>(a, worker, &run);
+			const int valid = min(half_rows, run.rows() - sub * half_rows); // rows of this subtile
+			if (warp == 0 && lane == 0 && from == 0 && !run.whole()) ac_job<kCtKT>(a, worker, &run);
 			if (valid <= 0) {
 				ring.skip(2 * (to_tile - from), stages);
 				continue;
 			}
-			// rows past the last one repeat it: their scores are masked alike, their outputs not stored
-			const int fr = run.tile * kCtR + sub * 128 + min(r, valid - 1);
+			// rows past the last one repeat its position: their scores are masked alike, their outputs not stored
+			const int fr = run.tile * a.R + sub * half_rows + min(r, valid - 1);
 			const int tok = a.group.div(fr), head = run.h * a.G + a.group.mod(fr);
 			const int pos = run.q.ctx - run.q.n + tok;
-			{
-				// Q: the warp reads its rows one after the other, 16 bytes per lane, all in flight together
-				const uint64_t src = (uint64_t)(run.q.row0 + tok) * a.q_stride + (uint64_t)head * HD;
-				constexpr int kUnits = HD / 8, kPer = 32 / kUnits; // 16-byte units of a row, rows per step
-				const int c = lane % kUnits;
-				uint4 u[32 / kPer];
-#pragma unroll
-				for (int i = 0; i < 32 / kPer; ++i) {
-					const uint64_t s = __shfl_sync(0xFFFFFFFFu, src, i * kPer + lane / kUnits);
-					u[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + s + c * 8));
-				}
-#pragma unroll
-				for (int i = 0; i < 32 / kPer; ++i)
-					*reinterpret_cast<uint4*>(qd + (size_t)(c >> 3) * kCtAtom + sw128_off(quarter * 32 + i * kPer + lane / kUnits, c & 7)) = u[i];
-				asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-				__syncwarp();
-				if (lane == 0) mbar_arrive(&bars[kCtQ + sub]);
-			}
 			const int lo = run.t.lo, hi = run.t.hi;
+			const int bot0 = a.window ? pos - a.window + 1 : 0; // the row's window (0: from the start)
 			float m = -INFINITY, l = 0.0f;
 			for (int i = from; i < to_tile; ++i) {
 				const int k0 = ac_tile_at(run.t, i) * kCtKT;
@@ -452,20 +493,51 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 				const int vstage = ring.stage;
 				const uint32_t vphase = ring.phase;
 				ring.next(stages);
+				// visible keys, a bit each: up to `top` and, under a window, from `bot` on or below the sinks' end
+				const int top = pos - k0, bot = bot0 - k0, sk = n_sink - k0;
+				const bool masked = __any_sync(0xFFFFFFFFu, top < kCtKT - 1 || (bot > 0 && sk < kCtKT));
+				const bool ragged = k0 + kCtKT > hi || (k0 < lo && min(k0 + kCtKT, lo) > n_sink);
 				ok = wait(kCtS + sub, s_par);
-				if (!ok) break;
+				if (__builtin_expect(!ok, 0)) break;
 				s_par ^= 1u;
 				tc_fence_after();
-				float v[kCtKT];
+				float v[4][32];
 #pragma unroll
-				for (int c = 0; c < kCtKT; c += 32) tmem_ld_32cols_nowait(ts + (uint32_t)c, v + c);
-				asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-				// V rows that no row of the item sees become zeros
-				if (k0 + kCtKT > hi || (k0 < lo && min(k0 + kCtKT, lo) > a.n_sink)) {
+				for (int q = 0; q < 4; ++q) tmem_ld_32(ts + (uint32_t)q * 32, v[q]);
+#pragma unroll
+				for (int q = 0; q < 4; ++q) tmem_ld_wait(v[q]);
+				if (__builtin_expect(masked, 0)) { // (edge code out of the loop's straight line: it is 4 KB of instructions)
+#pragma unroll
+					for (int q = 0; q < 4; ++q) { // bits tested with constants, so that no lane branches
+						const uint32_t w = low_bits(top + 1 - q * 32) & (~low_bits(bot - q * 32) | low_bits(sk - q * 32));
+#pragma unroll
+						for (int c = 0; c < 32; ++c) v[q][c] = (w & (1u << c)) ? v[q][c] : -INFINITY;
+					}
+				}
+				float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+				for (int c = 0; c < 32; c += 2)
+#pragma unroll
+					for (int q = 0; q < 4; ++q) m4[q] = fmaxf(m4[q], fmaxf(v[q][c], v[q][c + 1]));
+				const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
+				const bool grow = mt > m + kCtRescaleLog2 || (m == -INFINITY && mt != -INFINITY);
+				const float mn = grow ? mt : m;
+				if (__builtin_expect(__any_sync(0xFFFFFFFFu, grow && m != -INFINITY), 0)) {
+					// S is complete, so every earlier product is: O holds still
+					const float f = grow && m != -INFINITY ? ex2_approx(m - mn) : 1.0f;
+					l *= f;
+#pragma unroll 1
+					for (int c = 0; c < HD; c += 16) tmem_scale_16(to + (uint32_t)c, f);
+				}
+				m = mn;
+				const float mu = m == -INFINITY ? 0.0f : m; // nothing seen yet: 2^(-inf) = 0
+				const uint64_t mux2 = f2(-mu, -mu);
+				// V rows that no row of the item sees become zeros, ahead of P's first half
+				if (__builtin_expect(ragged, 0)) {
 					ok = wait(kCtFull + vstage, vphase);
 					if (!ok) break;
 					const int k = k0 + r;
-					if (k >= hi || (k < lo && k >= a.n_sink)) {
+					if (k >= hi || (k < lo && k >= n_sink)) {
 						uint4* row = reinterpret_cast<uint4*>(ring_s + (size_t)vstage * kTile + (r >> 3) * kGroup + (r & 7) * 128);
 #pragma unroll
 						for (int h = 0; h < kHalves; ++h)
@@ -474,55 +546,16 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 					}
 					asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 				}
-				// mask: keys above `top` and, under a window, those from the sinks to below `bot`
-				const int top = pos - k0, bot = a.window ? pos - a.window + 1 - k0 : 0, sk = a.n_sink - k0;
-				if (__any_sync(0xFFFFFFFFu, top < kCtKT - 1 || (bot > 0 && sk < kCtKT))) {
-#pragma unroll
-					for (int q = 0; q < 4; ++q) {
-						// a bit per key; tested with constants, so that no lane branches
-						const uint32_t w = low_bits(top + 1 - q * 32) & (~low_bits(bot - q * 32) | low_bits(sk - q * 32));
-#pragma unroll
-						for (int c = 0; c < 32; ++c) v[q * 32 + c] = (w & (1u << c)) ? v[q * 32 + c] : -INFINITY;
-					}
-				}
-				float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-				for (int c = 0; c < kCtKT; ++c) m4[c & 3] = fmaxf(m4[c & 3], v[c]);
-				const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
-				const bool grow = mt > m + kCtRescaleLog2 || (m == -INFINITY && mt != -INFINITY);
-				const float mn = grow ? mt : m;
-				if (i > from && __any_sync(0xFFFFFFFFu, grow && m != -INFINITY)) {
-					// S is complete, so every earlier product is: O holds still
-					const float f = grow && m != -INFINITY ? ex2_approx(m - mn) : 1.0f;
-					l *= f;
-#pragma unroll 1
-					for (int c = 0; c < HD; c += 32) {
-						float o[32];
-						tmem_ld_32cols(to + (uint32_t)c, o);
-#pragma unroll
-						for (int k = 0; k < 32; ++k) o[k] *= f;
-						tmem_st_32cols(to + (uint32_t)c, o);
-					}
-				}
-				m = mn;
-				const float mu = m == -INFINITY ? 0.0f : m; // nothing seen yet: 2^(-inf) = 0
-				const uint64_t sl2x2 = f2(sl2, sl2), mux2 = f2(-mu, -mu);
-				uint64_t sum[2] = {0, 0};
 #pragma unroll
 				for (int q = 0; q < 4; ++q) {
 					uint32_t pk[16];
 #pragma unroll
 					for (int c = 0; c < 16; ++c) {
-						const uint64_t x = f2_fma(f2(v[q * 32 + 2 * c], v[q * 32 + 2 * c + 1]), sl2x2, mux2);
+						const uint64_t x = f2_fma(f2(v[q][2 * c], v[q][2 * c + 1]), sl2x2, mux2);
 						float p0, p1;
-						if (c % 8 < kCtPolyOf8) {
-							ex2_poly2(x, p0, p1);
-						} else {
-							f2_split(x, p0, p1);
-							p0 = ex2_approx(p0);
-							p1 = ex2_approx(p1);
-						}
-						sum[c & 1] = f2_add(sum[c & 1], f2(p0, p1));
+						f2_split(x, p0, p1);
+						v[q][2 * c] = p0 = ex2_approx(p0);
+						v[q][2 * c + 1] = p1 = ex2_approx(p1);
 						pk[c] = pack_bf16(p0, p1);
 					}
 					tmem_st_16regs(ts + (uint32_t)q * 16, pk);
@@ -533,8 +566,14 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 						if (lane == 0) mbar_arrive(&bars[kCtP + sub * 2 + (q >> 1)]);
 					}
 				}
+				// the row's sum, while the products run
+				uint64_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+				for (int c = 0; c < 32; c += 2)
+#pragma unroll
+					for (int q = 0; q < 4; ++q) sum[q] = f2_add(sum[q], f2(v[q][c], v[q][c + 1]));
 				float s0, s1;
-				f2_split(f2_add(sum[0], sum[1]), s0, s1);
+				f2_split(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])), s0, s1);
 				l += s0 + s1;
 			}
 			if (!ok) break;
@@ -542,33 +581,41 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 			if (!ok) break;
 			o_par ^= 1u;
 			tc_fence_after();
-			float o[HD];
+			const bool whole = run.whole();
+			const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+			uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.out) + (uint64_t)(run.q.row0 + tok) * a.out_stride +
+			                                      (uint64_t)head * HD);
+			// a share of a divided item: [hd / 4][R] float4, so that a warp's stores are whole lines
+			float* part = a.part + (size_t)run.slot(worker) * ac_part_floats(a.R, HD);
+			const int pr = sub * half_rows + r;
+#pragma unroll 1
+			for (int c = 0; c < HD; c += 64) {
+				float o[2][32];
+				tmem_ld_32(to + (uint32_t)c, o[0]);
+				tmem_ld_32(to + (uint32_t)c + 32, o[1]);
+				tmem_ld_wait(o[0]);
+				tmem_ld_wait(o[1]);
+				if (r >= valid) continue;
+				if (whole) {
 #pragma unroll
-			for (int c = 0; c < HD; c += 32) tmem_ld_32cols_nowait(to + (uint32_t)c, o + c);
-			asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-			// a row that has seen nothing: its weights were 2^-126 at most, of whatever V holds
-			if (m == -INFINITY) l = 0.0f;
-			if (run.whole()) {
-				const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-				uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.out) + (uint64_t)(run.q.row0 + tok) * a.out_stride +
-				                                      (uint64_t)head * HD);
-				if (r < valid) {
+					for (int u = 0; u < 8; ++u) {
+						const float* x = &o[u >> 2][(u & 3) * 8];
+						dst[c / 8 + u] = make_uint4(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv),
+						                            pack_bf16(x[4] * inv, x[5] * inv), pack_bf16(x[6] * inv, x[7] * inv));
+					}
+				} else {
 #pragma unroll
-					for (int u = 0; u < HD / 8; ++u)
-						dst[u] = make_uint4(pack_bf16(o[8 * u] * inv, o[8 * u + 1] * inv), pack_bf16(o[8 * u + 2] * inv, o[8 * u + 3] * inv),
-						                    pack_bf16(o[8 * u + 4] * inv, o[8 * u + 5] * inv), pack_bf16(o[8 * u + 6] * inv, o[8 * u + 7] * inv));
+					for (int u = 0; u < 16; ++u) {
+						const float* x = &o[u >> 3][(u & 7) * 4];
+						reinterpret_cast<float4*>(part)[(size_t)(c / 4 + u) * a.R + pr] = make_float4(x[0], x[1], x[2], x[3]);
+					}
 				}
-			} else if (r < valid) {
-				// a share of a divided item: [hd / 4][256] float4, so that a warp's stores are whole lines
-				float* part = a.part + (size_t)run.slot(worker) * ac_part_floats(kCtR, HD);
-				const int pr = sub * 128 + r;
-#pragma unroll
-				for (int u = 0; u < HD / 4; ++u)
-					reinterpret_cast<float4*>(part)[(size_t)u * kCtR + pr] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
-				part[(size_t)kCtR * HD + pr] = m;
-				part[(size_t)kCtR * HD + kCtR + pr] = l;
 			}
-			tc_fence_before(); // the next item's first product overwrites O after this warpgroup's next P
+			if (!whole && r < valid) {
+				part[(size_t)a.R * HD + pr] = m;
+				part[(size_t)a.R * HD + a.R + pr] = l;
+			}
+			tc_fence_before(); // the next item's first product overwrites O behind this warpgroup's next P
 		}
 	}
 	tc_fence_before();

@@ -133,12 +133,16 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
 // mbar_wait timed by the SM's cycle counter: reading %globaltimer takes about a thousand cycles, which a
 // pipeline that waits at every tile pays each time a phase is not complete at once.  4e9 cycles are 2 s at
 // 2 GHz.
+// kSleepNs: pause between polls, for waits that are long and not on the critical path (a poll takes issue slots
+// from the warps that compute).
 constexpr long long kWaitLimitCycles = 4000000000ll;
+template <int kSleepNs = 0>
 __device__ __forceinline__ bool mbar_wait_cycles(uint64_t* bar, uint32_t parity, volatile int* abort, int* err)
 {
-	if (mbar_try_wait(bar, parity)) return true;
+	if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
 	const long long t0 = clock64();
 	for (uint32_t it = 1;; ++it) {
+		if (kSleepNs > 0) __nanosleep(kSleepNs);
 		if (mbar_try_wait(bar, parity)) return true;
 		if ((it & 63u) == 0) {
 			if (*abort) return false;
@@ -151,7 +155,15 @@ __device__ __forceinline__ bool mbar_wait_cycles(uint64_t* bar, uint32_t parity,
 	}
 }
 
-// 5-D tiled TMA load
+// 3-D and 5-D tiled TMA loads
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar, uint64_t policy)
+{
+	asm volatile(
+	    "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+	    " [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_u32(dst)),
+	    "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)), "l"(policy)
+	    : "memory");
+}
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4, uint64_t* bar,
                                             uint64_t policy)
 {
