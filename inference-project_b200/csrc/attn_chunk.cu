@@ -6,6 +6,7 @@
 #include <cstring>
 
 #include "k_attn_chunk.cuh"
+#include "k_attn_chunk_rows.cuh"
 #include "k_attn_chunk_tc.cuh"
 #include "launch.h"
 
@@ -17,7 +18,7 @@ u64 up256(u64 n) { return (n + 255) & ~255ull; }
 
 // One kernel's share of a call: the sequences with rows_min < rows <= rows_max rows per KV head.
 struct ChunkPass {
-	enum Kind { F32, TC } kind;
+	enum Kind { F32, Rows, TC } kind;
 	int rows_min, rows_max;
 	int workers, min_run;
 	int R;               // row tile
@@ -63,11 +64,26 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 		P->pass[P->n_pass++] = p;
 		return Success;
 	};
-	const u32 blk = kv->kv_block;
-	const u32 G = n_heads / kv->n_kv_heads;
-	if (kv->dtype == InfBF16 && G <= kCtRows && (kv->head_dim == 64 || kv->head_dim == 128) && (blk == 16 || blk == 32 || blk == 64 || blk == 128)) {
+	const u32 blk = kv->kv_block, G = n_heads / kv->n_kv_heads;
+	if (kv->dtype == InfBF16 && G <= kCtRows && (kv->head_dim == 64 || kv->head_dim == 128) &&
+	    (blk == 16 || blk == 32 || blk == 64 || blk == 128)) {
+		// Sequences of at most 16 rows per KV head go to the streaming kernel (HBM-bound, a warp per worker), longer
+		// ones to the tensor-core kernel, which reads K and V as fast but computes 128 rows whatever is there.
+		// Where sequences of max_new rows nearly fill the tokens no short one is left, and the tensor-core
+		// kernel takes all: the other launch would cost 3 us for nothing.
+		if (G <= (u32)kCrRows) {
+			ChunkPass r = {};
+			r.kind = ChunkPass::Rows;
+			r.rows_max = kCrRows;
+			r.R = kCrRows;
+			r.min_run = 4;
+			r.smem = attn_chunk_rows_smem((int)kv->head_dim, (int)n_seqs);
+			r.workers = sms * kCrWarps;
+			INF_TRY(add(r, (u64)std::min(n_seqs, n_tokens) * kv->n_kv_heads * (((u64)kv->pages_per_seq * blk + kCrKT - 1) / kCrKT + 1)));
+		}
 		ChunkPass t = {};
 		t.kind = ChunkPass::TC;
+		t.rows_min = G <= (u32)kCrRows ? kCrRows : 0;
 		t.rows_max = 0x7FFFFFFF;
 		t.R = (int)(2 * (kCtRows / G) * G); // whole tokens in each half
 		t.min_run = 2;
@@ -99,10 +115,10 @@ Error_t launch_tc(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
 	const u32 blk = (u32)a.blk, box = kCtKT / blk;
 	CUtensorMap q, k8, k1, v8, v1;
 	INF_TRY(tensor_map_q(&q, a.q, (u32)a.n_tokens, (u32)a.H, HD, a.q_stride, (u32)a.G, (u32)(kCtRows / a.G)));
-	INF_TRY(tensor_map_kv_groups(&k8, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
-	INF_TRY(tensor_map_kv_groups(&k1, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
-	INF_TRY(tensor_map_kv_groups(&v8, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box));
-	INF_TRY(tensor_map_kv_groups(&v1, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1));
+	INF_TRY(tensor_map_kv_groups(&k8, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box, blk / 8));
+	INF_TRY(tensor_map_kv_groups(&k1, a.kpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1, blk / 8));
+	INF_TRY(tensor_map_kv_groups(&v8, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, box, blk / 8));
+	INF_TRY(tensor_map_kv_groups(&v1, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1, blk / 8));
 	INF_TRY(allow_smem(k_attn_chunk_tc<HD>, 227 * 1024));
 	// the kernel's warpgroups trade registers within what it was launched with
 	static const int regs = [] {
@@ -111,6 +127,16 @@ Error_t launch_tc(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
 	}();
 	if (regs < kCtRegsLaunch) return fail(ErrorUnsupported, "inf_attn_chunk: built with %d registers a thread", regs);
 	return launch_pdl(k_attn_chunk_tc<HD>, dim3((unsigned)p.workers), dim3(kCtThreads), p.smem, st, q, k8, k1, v8, v1, a);
+}
+
+template <int HD>
+Error_t launch_rows(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
+{
+	CUtensorMap k, v;
+	INF_TRY(tensor_map_kv_groups(&k, a.kpool, HD, (u32)a.blk, (u32)a.KV, (u32)a.n_pages, 1, kCrKT / 8));
+	INF_TRY(tensor_map_kv_groups(&v, a.vpool, HD, (u32)a.blk, (u32)a.KV, (u32)a.n_pages, 1, kCrKT / 8));
+	INF_TRY(allow_smem(k_attn_chunk_rows<HD>, attn_chunk_rows_smem(HD, kAcMaxSeqs)));
+	return launch_pdl(k_attn_chunk_rows<HD>, dim3((unsigned)((p.workers + kCrWarps - 1) / kCrWarps)), dim3(kCrThreads), p.smem, st, k, v, a);
 }
 
 } // namespace
@@ -190,17 +216,33 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 		b.jobs = (int*)((uint8_t*)A.scratch + p.jobs_off);
 		return b;
 	};
+	// which of the two bf16 passes can have work
+	bool on[2] = {P.n_pass > 0, P.n_pass > 1};
+	if (P.n_pass == 2) {
+		const u64 slack = (u64)a.n_seqs * (u64)a.max_new - (u64)a.n_tokens; // rows missing to max_new in every sequence
+		on[1] = (u64)a.max_new * a.G > (u64)kCrRows;
+		on[0] = !on[1] || (u64)a.n_seqs * (u64)a.max_new < (u64)a.n_tokens || (slack + kCrRows / a.G) >= (u64)a.max_new;
+		if (!on[0]) P.pass[1].rows_min = 0;
+	}
+	int before = 0; // passes of this call that are running
 	for (int i = 0; i < P.n_pass; ++i) {
-		const AttnChunkArgs b = pass_args(P.pass[i]);
-		if (P.pass[i].kind == ChunkPass::TC) INF_TRY(a.hd == 64 ? launch_tc<64>(b, P.pass[i], st) : launch_tc<128>(b, P.pass[i], st));
-		else INF_TRY(kv->dtype == InfBF16 ? launch_f32<bf16>(b, P.pass[i], st) : launch_f32<float>(b, P.pass[i], st));
+		if (!on[i]) continue;
+		const ChunkPass& p = P.pass[i];
+		AttnChunkArgs b = pass_args(p);
+		// the second pass needs nothing of the first: it starts as soon as SMs are free, and waits at its end
+		b.late_wait = before > 0;
+		if (p.kind == ChunkPass::Rows) INF_TRY(a.hd == 64 ? launch_rows<64>(b, p, st) : launch_rows<128>(b, p, st));
+		else if (p.kind == ChunkPass::TC) INF_TRY(a.hd == 64 ? launch_tc<64>(b, p, st) : launch_tc<128>(b, p, st));
+		else INF_TRY(kv->dtype == InfBF16 ? launch_f32<bf16>(b, p, st) : launch_f32<float>(b, p, st));
+		++before;
 	}
 	for (int i = 0; i < P.n_pass; ++i) {
+		if (!on[i]) continue;
 		const ChunkPass& p = P.pass[i];
 		const AttnChunkArgs b = pass_args(p);
 		const dim3 grid((unsigned)p.workers, (unsigned)((p.R + 31) / 32));
-		INF_TRY(launch_pdl(kv->dtype == InfBF16 ? k_attn_chunk_combine<bf16> : k_attn_chunk_combine<float>, grid,
-		                   dim3(kAcCombineThreads), 0, st, b));
+		INF_TRY(launch_pdl(kv->dtype == InfBF16 ? k_attn_chunk_combine<bf16> : k_attn_chunk_combine<float>, grid, dim3(kAcCombineThreads),
+		                   0, st, b));
 	}
 	return Success;
 }

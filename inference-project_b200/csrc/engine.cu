@@ -230,13 +230,13 @@ Error_t tensor_map_q(CUtensorMap* m, const void* base, u32 tokens, u32 heads, u3
 	return Success;
 }
 
-Error_t tensor_map_kv_groups(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages)
+Error_t tensor_map_kv_groups(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages, u32 box_groups)
 {
 	PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
 	INF_TRY(tensor_map_encoder(&encode));
 	const cuuint64_t dims[5] = {64, (cuuint64_t)kv * blk, hd / 64, blk / 8, pages};
 	const cuuint64_t strides[4] = {(cuuint64_t)hd * 2, 128, (cuuint64_t)hd * 16, (cuuint64_t)kv * blk * hd * 2};
-	const cuuint32_t box[5] = {64, 8, hd / 64, blk / 8, box_pages};
+	const cuuint32_t box[5] = {64, 8, hd / 64, box_groups, box_pages};
 	const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
 	const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
 	                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

@@ -59,6 +59,7 @@ struct AttnChunkArgs {
 	int R;                         // rows of an item
 	int workers;
 	int min_run;                   // key tiles of a worker at least
+	int late_wait;                 // this kernel may run beside the one before it and waits for it at its end
 	float* part;                   // [2 * workers][hd + 2][R] partial O (unnormalised), max (log2 units), sum
 	int* jobs;                     // [workers][kAcJobInts]: the item that a worker begins and others end
 };
@@ -293,7 +294,8 @@ __host__ __device__ constexpr size_t ac_part_floats(int R, int hd) { return (siz
 // Joins the shares of every item that a cut divides: blockIdx.x is the worker that began it, blockIdx.y a
 // block of 32 rows.  A partial holds O as [hd / 4][R] float4, then the rows' max and sum.
 //   m = max_i m_i,  O = sum_i 2^(m_i - m) O_i,  l = sum_i 2^(m_i - m) l_i,  out = O / l
-// A lane owns a row, so that a warp's reads are whole lines; the eight warps share the head dims.
+// A lane owns a row and, where the item has fewer than 32, every 32 / rows-th share (reads of a row block are
+// whole lines, and a long context's many shares are read side by side); the warps share the head dims.
 constexpr int kAcCombineThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kAcCombineThreads) k_attn_chunk_combine(const AttnChunkArgs a)
@@ -303,36 +305,36 @@ __global__ void __launch_bounds__(kAcCombineThreads) k_attn_chunk_combine(const 
 	pdl_trigger();
 	const int w0 = blockIdx.x;
 	const int* j = a.jobs + (size_t)w0 * kAcJobInts;
-	const int rows = j[kAcJobRows];
-	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 32 + lane;
-	if (r >= rows) return;
+	const int rows = j[kAcJobRows] - (int)blockIdx.y * 32; // of this block
+	if (rows <= 0) return;
+	int wide = 1; // lanes of a row block: a power of two
+	while (wide < min(rows, kWarp)) wide <<= 1;
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = kWarp / wide;
+	const bool on = (lane & (wide - 1)) < rows;
+	const int r = (int)blockIdx.y * 32 + (on ? lane & (wide - 1) : 0), first = w0 + lane / wide;
 	const int last = j[kAcJobLast], hd4 = a.hd / 4;
 	const size_t pf = ac_part_floats(R, a.hd);
 	// the beginner's share is its second slot, the others' their first
 	auto part = [&](int w) { return a.part + (size_t)(2 * w + (w == w0 ? 1 : 0)) * pf; };
 	float m = -INFINITY;
 #pragma unroll 4
-	for (int w = w0; w <= last; ++w) m = fmaxf(m, part(w)[(size_t)R * a.hd + r]);
+	for (int w = first; w <= last; w += step) m = fmaxf(m, part(w)[(size_t)R * a.hd + r]);
+	for (int o = wide; o < kWarp; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
 	if (m == -INFINITY) m = 0.0f; // every share without keys: weights of 2^-inf = 0
-	float l = 0.0f;
-#pragma unroll 4
-	for (int w = w0; w <= last; ++w) {
-		const float* p = part(w) + (size_t)R * a.hd + r;
-		l = fmaf(exp2f(p[0] - m), p[R], l);
-	}
-	const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 	const int fr = j[kAcJobRow] + r;
 	T* out = reinterpret_cast<T*>(a.out) + (size_t)(j[kAcJobSeq] + a.group.div(fr)) * a.out_stride +
 	         (size_t)(j[kAcJobHead] * a.G + a.group.mod(fr)) * a.hd;
 	constexpr int kWarps = kAcCombineThreads / kWarp, kCols = 4;
 	for (int c0 = warp * kCols; c0 < hd4; c0 += kWarps * kCols) {
 		float4 o[kCols];
+		float l = 0.0f;
 #pragma unroll
 		for (int c = 0; c < kCols; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
-		for (int w = w0; w <= last; ++w) {
+		for (int w = first; w <= last; w += step) {
 			const float* p = part(w);
 			const float f = exp2f(p[(size_t)R * a.hd + r] - m);
+			l = fmaf(f, p[(size_t)R * a.hd + R + r], l);
 #pragma unroll
 			for (int c = 0; c < kCols; ++c) {
 				if (c0 + c >= hd4) continue;
@@ -343,6 +345,18 @@ __global__ void __launch_bounds__(kAcCombineThreads) k_attn_chunk_combine(const 
 				o[c].w = fmaf(f, v.w, o[c].w);
 			}
 		}
+		for (int s = wide; s < kWarp; s <<= 1) {
+			l += __shfl_xor_sync(0xFFFFFFFFu, l, s);
+#pragma unroll
+			for (int c = 0; c < kCols; ++c) {
+				o[c].x += __shfl_xor_sync(0xFFFFFFFFu, o[c].x, s);
+				o[c].y += __shfl_xor_sync(0xFFFFFFFFu, o[c].y, s);
+				o[c].z += __shfl_xor_sync(0xFFFFFFFFu, o[c].z, s);
+				o[c].w += __shfl_xor_sync(0xFFFFFFFFu, o[c].w, s);
+			}
+		}
+		if (!on || lane >= wide) continue;
+		const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
 		for (int c = 0; c < kCols; ++c) {
 			if (c0 + c >= hd4) continue;

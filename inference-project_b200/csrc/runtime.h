@@ -41,10 +41,10 @@ Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv,
 // Rows of `heads` heads of hd, `stride` elements apart, as a 3-D tensor (dim, head, token) with boxes of 64 dims x
 // box_heads x box_tokens, SWIZZLE_128B.
 Error_t tensor_map_q(CUtensorMap* m, const void* base, u32 tokens, u32 heads, u32 hd, u64 stride, u32 box_heads, u32 box_tokens);
-// A K or V pool as a 5-D tensor (64 dims of a row, 8 rows, head_dim / 64, blk / 8, page), SWIZZLE_128B: a box is one
-// head of box_pages consecutive pages, and lands as [pages * blk / 8][head_dim / 64][8 rows x 128 bytes], an even
+// A K or V pool as a 5-D tensor (64 dims of a row, 8 rows, head_dim / 64, blk / 8, page), SWIZZLE_128B: a box is
+// box_groups 8-row groups of one head of box_pages consecutive pages, and lands as [box_pages * box_groups][head_dim / 64][8 rows x 128 bytes], an even
 // stride between the 8-row groups of all pages.  The second coordinate is head * blk.
-Error_t tensor_map_kv_groups(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages);
+Error_t tensor_map_kv_groups(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages, u32 box_groups);
 
 // Whether inf_set_sampling turned sampling on for this model (false for NULL).
 bool model_sampling_on(const Model* m);
