@@ -103,6 +103,22 @@ __device__ __forceinline__ void unpack_unit(const uint4& u, float* out, const fl
 	out[2] = __uint_as_float(u.z); out[3] = __uint_as_float(u.w);
 }
 
+// floats into one 16-byte unit, rounded to nearest even
+__device__ __forceinline__ uint4 pack_unit(const float* v, bf16*)
+{
+	uint32_t w[4];
+#pragma unroll
+	for (int i = 0; i < 4; ++i) {
+		const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+		memcpy(&w[i], &b, 4);
+	}
+	return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack_unit(const float* v, float*)
+{
+	return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+
 // ---- programmatic dependent launch ----------------------------------------------------
 // Pre-wait code may only read memory that no kernel of the same step writes (weights).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -357,14 +357,22 @@ __global__ void __launch_bounds__(kAcCombineThreads) k_attn_chunk_combine(const 
 		}
 		if (!on || lane >= wide) continue;
 		const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+		// a row's 16 dims as 16-byte stores (single values, each lane in another row, had taken 50 us for 39 MB
+		// of shares); head_dim is a multiple of 16 bytes, so a last short block is whole units too
 #pragma unroll
-		for (int c = 0; c < kCols; ++c) {
-			if (c0 + c >= hd4) continue;
-			T* d = out + 4 * (c0 + c);
-			Store<T>::put(d, o[c].x * inv);
-			Store<T>::put(d + 1, o[c].y * inv);
-			Store<T>::put(d + 2, o[c].z * inv);
-			Store<T>::put(d + 3, o[c].w * inv);
+		for (int u = 0; u < (int)(kCols * 4 * sizeof(T) / 16); ++u) {
+			constexpr int kPer = 16 / sizeof(T) / 4; // float4 per unit
+			if (c0 + u * kPer >= hd4) continue;
+			float x[16 / sizeof(T)];
+#pragma unroll
+			for (int c = 0; c < kPer; ++c) {
+				const float4& v = o[u * kPer + c];
+				x[4 * c] = v.x * inv;
+				x[4 * c + 1] = v.y * inv;
+				x[4 * c + 2] = v.z * inv;
+				x[4 * c + 3] = v.w * inv;
+			}
+			*reinterpret_cast<uint4*>(out + 4 * (c0 + u * kPer)) = pack_unit(x, (T*)nullptr);
 		}
 	}
 }

@@ -18,22 +18,6 @@ namespace inf {
 constexpr int kQnThreads = 256;
 constexpr int kQnBatch = 4; // heads in flight per group
 
-// floats into one 16-byte unit, rounded to nearest even
-__device__ __forceinline__ uint4 pack_unit(const float* v, bf16*)
-{
-	uint32_t w[4];
-#pragma unroll
-	for (int i = 0; i < 4; ++i) {
-		const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-		memcpy(&w[i], &b, 4);
-	}
-	return make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ uint4 pack_unit(const float* v, float*)
-{
-	return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-}
-
 struct QkNormRopeArgs {
 	const uint8_t* qkv;
 	uint8_t* q_out;
