@@ -4,8 +4,8 @@
 // heads of a KV group) and key tiles of 128 positions.  The rows are two subtiles of up to 128, each with its
 // own warpgroup, so that one subtile's exponentials run while the tensor cores work on the other's products:
 //   warps 0-3, 4-7  a thread per row of subtile 0, 1: per key tile S from tensor memory into registers, mask,
-//                   running max, P = 2^(s scale - m) as bf16 back into the same tensor-memory columns in two
-//                   halves, then the row's sum (off the path to the next product); O / sum at the end
+//                   running max, P = 2^(s scale - m) as bf16 back into the same tensor-memory columns, then
+//                   the row's sum (off the path to the next product); O / sum at the end
 //   warps 8, 10     TMA producers of K and of V tiles into one ring (no multicast): a 5-D box per page, [8-row
 //                   group][64 head dims][8 x 128 bytes], or one for the whole tile where the page ids are
 //                   consecutive
@@ -49,8 +49,8 @@ enum CtBar : int {
 	kCtQ = 2 * kCtMaxStages,              // [2] Q of the subtile loaded
 	kCtQFree = kCtQ + 2,                  // [2] the item's last S done with it
 	kCtS = kCtQFree + 2,                  // [2] S ready
-	kCtP = kCtS + 2,                      // [2][2] P's halves written (4 warps arrive)
-	kCtO = kCtP + 4,                      // [2] the item's last product done
+	kCtP = kCtS + 2,                      // [2] P written (4 warps arrive)
+	kCtO = kCtP + 2,                      // [2] the item's last product done
 	kCtDrain = kCtO + 2,
 	kCtBars = kCtDrain + 1
 };
@@ -335,17 +335,16 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 				          db + (uint32_t)((k >> 2) * 64 + (k & 3) * 2), idesc_s, k > 0 ? 1u : 0u);
 			umma_commit(&bars[kCtS + sub]);
 		};
-		auto mma_pv = [&](int sub, uint32_t stage, int half, uint32_t acc) {
+		auto mma_pv = [&](int sub, uint32_t stage, uint32_t acc) {
 			const uint64_t dv = umma_desc_sw128_lbo(ra + stage * kTile, 1024, kGroup);
 			const uint32_t pa = tm + (uint32_t)sub * kCtKT, od = tm + 2 * kCtKT + (uint32_t)(sub * HD);
 #pragma unroll
-			for (int k = half * 4; k < half * 4 + 4; ++k)
+			for (int k = 0; k < kCtKT / 16; ++k)
 				umma_bf16_ts(od, pa + (uint32_t)k * 8, dv + (uint32_t)(k * 2 * kGroup / 16), idesc_o, k > 0 ? 1u : acc);
 		};
-		bool ok = true;
-		for (; ok && !run.done(); run.next(a, pre)) {
-			const int n = run.to() - run.from();
-			const int subs = run.rows() > (a.R >> 1) ? 2 : 1;
+		bool ok = true, busy = !run.done();
+		int n = busy ? run.to() - run.from() : 0, subs = busy && run.rows() > (a.R >> 1) ? 2 : 1;
+		while (ok && busy) {
 			// S of the first tile
 			uint32_t ks = uniform((uint32_t)r.stage);
 			ok = wait(kCtFull + (int)ks, r.phase);
@@ -365,6 +364,10 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 			}
 			if (!ok) break;
 			r.next(stages);
+			// the next item, found while the softmax warps work
+			run.next(a, pre);
+			busy = !run.done();
+			const int next_n = busy ? run.to() - run.from() : 0, next_subs = busy && run.rows() > (a.R >> 1) ? 2 : 1;
 			for (int j = 0; ok && j < n; ++j) {
 				// V of this tile and K of the next are waited for ahead of P, so that nothing but the issue
 				// stands between P's second half and the next S
@@ -383,17 +386,12 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 #pragma unroll
 				for (int sub = 0; sub < 2; ++sub) {
 					if (!ok || sub >= subs) break;
-					ok = wait(kCtP + sub * 2, p_par[sub]);
-					if (!ok) break;
-					tc_fence_after();
-					if (elect_one()) mma_pv(sub, vs, 0, acc);
-					__syncwarp();
-					ok = wait(kCtP + sub * 2 + 1, p_par[sub]);
+					ok = wait(kCtP + sub, p_par[sub]);
 					if (!ok) break;
 					p_par[sub] ^= 1u;
 					tc_fence_after();
 					if (elect_one()) {
-						mma_pv(sub, vs, 1, 1u);
+						mma_pv(sub, vs, acc);
 						if (more) {
 							mma_s(sub, ks);
 							if (last_s) umma_commit(&bars[kCtQFree + sub]);
@@ -408,6 +406,8 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 					__syncwarp();
 				}
 			}
+			n = next_n;
+			subs = next_subs;
 		}
 		// every product is done before tensor memory is freed, whatever ended the loop
 		if (elect_one()) umma_commit(&bars[kCtDrain]);
@@ -472,12 +472,13 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 			return (bool)__all_sync(0xFFFFFFFFu, w);
 		};
 		if (warp == 0 && lane == 0) ac_job<kCtKT>(a, worker, nullptr);
-		for (; ok && !run.done(); run.next(a, pre)) {
+		while (ok && !run.done()) {
 			const int from = run.from(), to_tile = run.to();
 			const int valid = min(half_rows, run.rows() - sub * half_rows); // rows of this subtile
 			if (warp == 0 && lane == 0 && from == 0 && !run.whole()) ac_job<kCtKT>(a, worker, &run);
 			if (valid <= 0) {
 				ring.skip(2 * (to_tile - from), stages);
+				run.next(a, pre);
 				continue;
 			}
 			// rows past the last one repeat its position: their scores are masked alike, their outputs not stored
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 #pragma unroll
 						for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-							for (int c = 0; c < 8; ++c) row[h * 64 + c] = make_uint4(0, 0, 0, 0);
+							for (int c = 0; c < 8; ++c) row[h * 64 + ((c + lane) & 7)] = make_uint4(0, 0, 0, 0); // eight lanes, eight bank groups
 					}
 					asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 				}
@@ -559,13 +560,11 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 						pk[c] = pack_bf16(p0, p1);
 					}
 					tmem_st_16regs(ts + (uint32_t)q * 16, pk);
-					if (q & 1) {
-						asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-						tc_fence_before();
-						__syncwarp();
-						if (lane == 0) mbar_arrive(&bars[kCtP + sub * 2 + (q >> 1)]);
-					}
 				}
+				asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+				tc_fence_before();
+				__syncwarp();
+				if (lane == 0) mbar_arrive(&bars[kCtP + sub]);
 				// the row's sum, while the products run
 				uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -577,17 +576,19 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 				l += s0 + s1;
 			}
 			if (!ok) break;
-			ok = wait(kCtO + sub, o_par);
-			if (!ok) break;
-			o_par ^= 1u;
-			tc_fence_after();
+			// where O goes, and the next item, found while the last product runs
 			const bool whole = run.whole();
-			const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 			uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.out) + (uint64_t)(run.q.row0 + tok) * a.out_stride +
 			                                      (uint64_t)head * HD);
 			// a share of a divided item: [hd / 4][R] float4, so that a warp's stores are whole lines
 			float* part = a.part + (size_t)run.slot(worker) * ac_part_floats(a.R, HD);
 			const int pr = sub * half_rows + r;
+			const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+			run.next(a, pre);
+			ok = wait(kCtO + sub, o_par);
+			if (!ok) break;
+			o_par ^= 1u;
+			tc_fence_after();
 #pragma unroll 1
 			for (int c = 0; c < HD; c += 64) {
 				float o[2][32];
