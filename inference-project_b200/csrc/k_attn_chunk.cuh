@@ -388,10 +388,10 @@ constexpr int kAfKT = 32;
 constexpr int kAfThreads = 128;
 constexpr int kAfRows = kAfR / (kAfThreads / kWarp); // rows per warp
 
-// q [16][hd], K or V [32][hd + 4], P [16][32]
+// q [16][hd], K and V [32][hd + 4] each, P [16][32]
 __host__ __device__ constexpr size_t attn_chunk_f32_smem(int hd, int n_seqs)
 {
-	return ((size_t)kAfR * hd + (size_t)kAfKT * (hd + 4) + kAfR * kAfKT) * 4 + (size_t)(n_seqs + 1) * 4;
+	return ((size_t)kAfR * hd + (size_t)2 * kAfKT * (hd + 4) + kAfR * kAfKT) * 4 + (size_t)(n_seqs + 1) * 4;
 }
 
 // VPL: groups of 4 head dims per lane (head_dim <= 128 VPL)
@@ -403,8 +403,9 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 	pdl_trigger();
 	const int hd = a.hd, ld = hd + 4, hd4 = hd / 4;
 	float* q_s = af_smem;                 // [16][hd], scaled to log2 units
-	float* kv_s = q_s + kAfR * hd;        // [32][ld]
-	float* p_s = kv_s + kAfKT * ld;       // [16][32]
+	float* k_s = q_s + kAfR * hd;         // [32][ld]
+	float* v_s = k_s + kAfKT * ld;        // [32][ld]
+	float* p_s = v_s + kAfKT * ld;        // [16][32]
 	uint32_t* pre = reinterpret_cast<uint32_t*>(p_s + kAfR * kAfKT);
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, worker = blockIdx.x;
 	ac_prefix<kAfKT>(a, pre);
@@ -445,35 +446,37 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 		}
 		for (int kt = run.from(); kt < run.to(); ++kt) {
 			const int k0 = ac_tile_at(t, kt) * kAfKT;
-			// one pool's 32 rows of the tile; rows that no row of the item sees are zeros, so that nothing
-			// they hold reaches a sum
-			auto stage = [&](const void* pool) {
-				for (int u = threadIdx.x; u < kAfKT * (hd / V); u += kAfThreads) {
-					const int k = k0 + u / (hd / V), c = u % (hd / V);
-					uint4 x = make_uint4(0, 0, 0, 0);
-					if (k < t.hi && (k >= t.lo || k < a.n_sink)) {
-						const int page = a.table[(size_t)run.q.slot * a.pages_per_seq + k / a.blk];
-						if (page >= 0 && page < a.n_pages)
-							x = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(pool) +
-							                                   (((size_t)page * a.KV + run.h) * a.blk + k % a.blk) * hd)[c];
-						else
-							report_err(a.status, kDevKvRange);
+			// the tile's 32 rows of K and of V; rows that no row of the item sees are zeros, so that nothing they
+			// hold reaches a sum
+			__syncthreads(); // the tile before it is read
+			for (int u = threadIdx.x; u < kAfKT * (hd / V); u += kAfThreads) {
+				const int k = k0 + u / (hd / V), c = u % (hd / V);
+				uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+				if (k < t.hi && (k >= t.lo || k < a.n_sink)) {
+					const int page = a.table[(size_t)run.q.slot * a.pages_per_seq + k / a.blk];
+					if (page >= 0 && page < a.n_pages) {
+						const size_t at = (((size_t)page * a.KV + run.h) * a.blk + k % a.blk) * hd;
+						x[0] = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.kpool) + at)[c];
+						x[1] = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.vpool) + at)[c];
+					} else {
+						report_err(a.status, kDevKvRange);
 					}
+				}
+#pragma unroll
+				for (int kv = 0; kv < 2; ++kv) {
 					float f[V];
-					unpack_unit(x, f, (const T*)nullptr);
+					unpack_unit(x[kv], f, (const T*)nullptr);
 #pragma unroll
 					for (int i = 0; i < V; i += 4)
-						*reinterpret_cast<float4*>(kv_s + (size_t)(k - k0) * ld + c * V + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+						*reinterpret_cast<float4*>((kv ? v_s : k_s) + (size_t)(k - k0) * ld + c * V + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
 				}
-			};
-			__syncthreads();
-			stage(a.kpool);
+			}
 			__syncthreads();
 			float sc[kAfRows];
 #pragma unroll
 			for (int i = 0; i < kAfRows; ++i) sc[i] = 0.0f;
 			for (int d = 0; d < hd; d += 4) {
-				const float4 kk = *reinterpret_cast<const float4*>(kv_s + (size_t)lane * ld + d);
+				const float4 kk = *reinterpret_cast<const float4*>(k_s + (size_t)lane * ld + d);
 #pragma unroll
 				for (int i = 0; i < kAfRows; ++i) {
 					const float4 qq = *reinterpret_cast<const float4*>(q_s + (warp * kAfRows + i) * hd + d);
@@ -499,9 +502,7 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 					o[i][v].w *= f;
 				}
 			}
-			__syncthreads(); // K is read, P written
-			stage(a.vpool);
-			__syncthreads();
+			__syncwarp(); // the warp's own rows of P
 			for (int k = 0; k < kAfKT; k += 4) {
 				float4 p[kAfRows];
 #pragma unroll
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 					if (c >= hd4) continue;
 #pragma unroll
 					for (int kk = 0; kk < 4; ++kk) {
-						const float4 x = *reinterpret_cast<const float4*>(kv_s + (size_t)(k + kk) * ld + c * 4);
+						const float4 x = *reinterpret_cast<const float4*>(v_s + (size_t)(k + kk) * ld + c * 4);
 #pragma unroll
 						for (int i = 0; i < kAfRows; ++i) {
 							const float w = kk == 0 ? p[i].x : kk == 1 ? p[i].y : kk == 2 ? p[i].z : p[i].w;

@@ -73,20 +73,27 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 	const uint64_t pol = policy_evict_first(); // read once
 	const int blk = a.blk;
 	int load_i = run.done() ? 0 : run.from(), issued = 0, stage_in = 0;
+	// page of the next tile to copy (-1: the tile of an item that sees nothing), read one copy ahead: a table
+	// entry takes as long to arrive as a tile's arithmetic
+	auto look = [&]() {
+		if (load.done()) return -1;
+		const int k0 = ac_tile_at(load.t, load_i) * kCrKT;
+		return k0 < load.t.hi ? a.table[(size_t)load.q.slot * a.pages_per_seq + k0 / blk] : -1;
+	};
+	int ahead = look();
 	auto fetch = [&]() { // the whole warp; no-op behind the run's end
 		if (load.done()) return;
 		const int k0 = ac_tile_at(load.t, load_i) * kCrKT;
-		const bool seen = k0 < load.t.hi; // an item that sees nothing has one empty tile
-		int page = seen ? a.table[(size_t)load.q.slot * a.pages_per_seq + k0 / blk] : 0;
-		if (seen && (page < 0 || page >= a.n_pages)) {
-			if (lane == 0) report_err(a.status, kDevKvRange);
+		int page = ahead;
+		if (page < 0 || page >= a.n_pages) {
+			if (k0 < load.t.hi && lane == 0) report_err(a.status, kDevKvRange);
 			page = 0;
 		}
 		page = (int)__shfl_sync(0xFFFFFFFFu, page, 0);
 		const int st = __shfl_sync(0xFFFFFFFFu, stage_in, 0), head_row = __shfl_sync(0xFFFFFFFFu, load.h * blk, 0);
-		const int group = __shfl_sync(0xFFFFFFFFu, (k0 % blk) >> 3, 0);
+		const int group = __shfl_sync(0xFFFFFFFFu, (k0 & (blk - 1)) >> 3, 0); // blk is a power of two here
 		uint8_t* dst = ring + (uint32_t)st * 2 * kTile;
-		if (lane == 0) {
+		if (elect_one()) {
 			mbar_arrive_expect_tx(&bars[st], 2 * kTile);
 			tma_load_5d(dst, &tm_k, 0, head_row, 0, group, page, &bars[st], pol);
 			tma_load_5d(dst + kTile, &tm_v, 0, head_row, 0, group, page, &bars[st], pol);
@@ -98,6 +105,7 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 			load.next(a, pre);
 			if (!load.done()) load_i = load.from();
 		}
+		ahead = look();
 	};
 	for (int i = 0; i < kStages; ++i) fetch();
 

@@ -119,22 +119,6 @@ __device__ __forceinline__ void tmem_st_16regs(uint32_t taddr, const uint32_t (&
 	    : "memory");
 }
 
-// One lane of a converged warp, and a value that is the same in all of them, from lane 0: operands that the
-// compiler knows to be uniform go to the tensor-core and copy instructions straight from uniform registers.
-// Issued from inside a divergent branch, with operands moved over one by one, eight products took about
-// 1000 cycles to issue for 512 of work.
-__device__ __forceinline__ bool elect_one()
-{
-	uint32_t ok;
-	asm volatile(
-	    "{\n\t.reg .pred p;\n\t"
-	    "elect.sync _|p, 0xFFFFFFFF;\n\t"
-	    "selp.u32 %0, 1, 0, p;\n\t}"
-	    : "=r"(ok));
-	return ok != 0;
-}
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
-
 // the n lowest bits (none for n <= 0, all from 32 on)
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
 

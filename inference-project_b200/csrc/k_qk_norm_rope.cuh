@@ -6,9 +6,10 @@
 //
 // Bound by HBM: every element is read once and written once.  A group of lanes owns a head, a lane the
 // 16-byte units u and u + units/2 of it, so both partners of a rotation are in one lane and the only
-// exchange is the sum of squares (3 shuffles for head_dim 128 in bf16: 8 lanes x 2 units).  A group goes
-// through several heads of its token, four at a time with their loads in flight together, and keeps
-// the token's cos and sin, which are as many bytes as two bf16 heads, in registers.
+// exchange is the sum of squares (3 shuffles for head_dim 128 in bf16: 8 lanes x 2 units).  A warp goes
+// through the heads of one token, its groups side by side, and keeps the products of gain, cos and sin in
+// registers: per element that leaves the unpacking, the square, one multiply-add and the scale, which the
+// SMs issue in about half of the time that HBM takes.
 #pragma once
 
 #include "common.cuh"
@@ -16,7 +17,7 @@
 namespace inf {
 
 constexpr int kQnThreads = 256;
-constexpr int kQnBatch = 4; // heads in flight per group
+constexpr int kQnBatch = 2; // heads in flight per group
 
 struct QkNormRopeArgs {
 	const uint8_t* qkv;
@@ -29,7 +30,7 @@ struct QkNormRopeArgs {
 	const int* tok_slot;
 	const int* tok_pos;
 	int* status;
-	float eps, gain_offset;
+	float eps, gain_offset, inv_hd;
 	int n_pos;
 	uint32_t n_tokens;
 	int H, KV, hd, blk;
@@ -38,126 +39,138 @@ struct QkNormRopeArgs {
 	const int* table;
 	int n_slots, pages_per_seq, n_pages;
 	int lanes;      // lanes per head, a power of two >= units / 2 / VP
-	int chunk;      // heads per group
-	int chunks;     // groups per token
+	int chunk;      // heads per warp
+	int chunks;     // warps per token
 };
 
-// VP: unit pairs per lane (1, or 2 for rows of more than 32 unit pairs)
+// VP: unit pairs per lane (1, or 2 for rows of more than 32 unit pairs).  Three CTAs an SM: 47 us for 8199 rows of
+// 48 x 128 bf16 (4.4 TB/s), against 52 with two CTAs and 128 registers and 49 with four and spills.
 template <typename T, int VP>
-__global__ void __launch_bounds__(kQnThreads) k_qk_norm_rope_rows(const QkNormRopeArgs a)
+__global__ void __launch_bounds__(kQnThreads, VP == 1 ? 3 : 1) k_qk_norm_rope_rows(const QkNormRopeArgs a)
 {
 	constexpr int V = Store<T>::kVec; // elements per unit
 	pdl_wait();
 	pdl_trigger();
-	const uint64_t thread = (uint64_t)blockIdx.x * kQnThreads + threadIdx.x;
-	const uint64_t group = thread / (uint32_t)a.lanes;
-	const int gl = (int)(thread % (uint32_t)a.lanes);
-	const uint64_t token = group / (uint32_t)a.chunks;
-	// the shuffles below name the whole warp: no thread leaves before the end
-	bool on = token < a.n_tokens;
-	const int slot = on ? a.tok_slot[token] : -1;
-	const int pos = on ? a.tok_pos[token] : 0;
-	on = on && slot >= 0; // a negative slot is padding
-	const int page_i = on ? pos / a.blk : 0;
-	if (on && (slot >= a.n_slots || pos < 0 || pos >= a.n_pos || page_i >= a.pages_per_seq)) {
-		if (gl == 0) report_err(a.status, kDevKvRange);
-		on = false;
+	const int lane = threadIdx.x & 31, gl = lane & (a.lanes - 1), grp = lane / a.lanes, groups = kWarp / a.lanes;
+	const uint64_t w = (uint64_t)blockIdx.x * (kQnThreads / kWarp) + threadIdx.x / kWarp;
+	const uint64_t token = w / (uint32_t)a.chunks; // a warp: `chunk` heads of one token
+	if (token >= a.n_tokens) return;
+	const int slot = a.tok_slot[token], pos = a.tok_pos[token];
+	if (slot < 0) return; // padding
+	const int page_i = pos / a.blk;
+	if (slot >= a.n_slots || pos < 0 || pos >= a.n_pos || page_i >= a.pages_per_seq) {
+		if (lane == 0) report_err(a.status, kDevKvRange);
+		return;
 	}
 	const int heads = a.H + 2 * a.KV;
-	const int h0 = (int)(group % (uint32_t)a.chunks) * a.chunk, h1 = min(heads, h0 + a.chunk);
-	const bool writes = on && h1 > a.H;
+	const int h0 = (int)(w % (uint32_t)a.chunks) * a.chunk, h1 = min(heads, h0 + a.chunk);
+	const bool writes = h1 > a.H;
 	const int page = writes ? a.table[(size_t)slot * a.pages_per_seq + page_i] : 0;
 	const bool page_ok = page >= 0 && page < a.n_pages;
-	if (writes && !page_ok && gl == 0) report_err(a.status, kDevKvRange);
+	if (writes && !page_ok && lane == 0) report_err(a.status, kDevKvRange);
 	const int half_units = a.hd / V / 2, half = a.hd / 2;
-	float c[VP][V], s[VP][V];
-	bool mine[VP];
-#pragma unroll
-	for (int p = 0; p < VP; ++p) {
-		const int u = gl + p * a.lanes;
-		mine[p] = on && u < half_units;
-#pragma unroll
-		for (int i = 0; i < V; i += 4) {
-			float4 cc = make_float4(1.f, 1.f, 1.f, 1.f), ss = make_float4(0.f, 0.f, 0.f, 0.f);
-			if (mine[p]) {
-				cc = *reinterpret_cast<const float4*>(a.rope_cos + (size_t)pos * half + u * V + i);
-				ss = *reinterpret_cast<const float4*>(a.rope_sin + (size_t)pos * half + u * V + i);
-			}
-			c[p][i] = cc.x; c[p][i + 1] = cc.y; c[p][i + 2] = cc.z; c[p][i + 3] = cc.w;
-			s[p][i] = ss.x; s[p][i + 1] = ss.y; s[p][i + 2] = ss.z; s[p][i + 3] = ss.w;
-		}
-	}
 	const uint8_t* row = a.qkv + token * a.qkv_stride;
 	const uint32_t head_bytes = (uint32_t)a.hd * sizeof(T);
 	const uint64_t slab = ((uint64_t)page * a.KV * a.blk + pos % a.blk) * head_bytes; // head 0's row of the page
-	for (int hb = h0; hb < h0 + a.chunk; hb += kQnBatch) { // the same trips in every group
-		uint4 lo[kQnBatch][VP], hi[kQnBatch][VP];
+	bool mine[VP];
 #pragma unroll
-		for (int b = 0; b < kQnBatch; ++b)
+	for (int p = 0; p < VP; ++p) mine[p] = gl + p * a.lanes < half_units;
+	// the warp's heads in three kinds: queries, keys, values; its groups take them in turn
+#pragma unroll 1
+	for (int kind = 0; kind < 3; ++kind) {
+		const int from = max(h0, kind == 0 ? 0 : kind == 1 ? a.H : a.H + a.KV);
+		const int to = min(h1, kind == 0 ? a.H : kind == 1 ? a.H + a.KV : heads);
+		if (from >= to) continue;
+		// with g = offset + gain: out_i = inv (x_i g_i cos_i - x_(i+h) g_(i+h) sin_i), the other half alike
+		float ac[VP][V], bs[VP][V], bc[VP][V], as[VP][V];
+		const T* gain = reinterpret_cast<const T*>(kind == 0 ? a.q_gain : a.k_gain);
 #pragma unroll
-			for (int p = 0; p < VP; ++p) {
-				lo[b][p] = hi[b][p] = make_uint4(0, 0, 0, 0);
-				if (mine[p] && hb + b < h1) {
-					const uint4* src = reinterpret_cast<const uint4*>(row + (size_t)(hb + b) * head_bytes);
-					lo[b][p] = src[gl + p * a.lanes];
-					hi[b][p] = src[gl + p * a.lanes + half_units];
+		for (int p = 0; p < VP; ++p) {
+			const int u = gl + p * a.lanes;
+			float g0[V], g1[V];
+#pragma unroll
+			for (int i = 0; i < V; ++i) g0[i] = g1[i] = 1.0f;
+			if (kind < 2 && gain && mine[p]) {
+				unpack_unit(reinterpret_cast<const uint4*>(gain)[u], g0, (const T*)nullptr);
+				unpack_unit(reinterpret_cast<const uint4*>(gain)[u + half_units], g1, (const T*)nullptr);
+#pragma unroll
+				for (int i = 0; i < V; ++i) {
+					g0[i] += a.gain_offset;
+					g1[i] += a.gain_offset;
 				}
 			}
 #pragma unroll
-		for (int b = 0; b < kQnBatch; ++b) {
-			const int h = hb + b;
-			const bool is_q = h < a.H, is_v = h >= a.H + a.KV;
-			float x[VP][V], y[VP][V];
-			float ss = 0.0f;
+			for (int i = 0; i < V; i += 4) {
+				float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+				if (kind < 2 && mine[p]) {
+					c = *reinterpret_cast<const float4*>(a.rope_cos + (size_t)pos * half + u * V + i);
+					s = *reinterpret_cast<const float4*>(a.rope_sin + (size_t)pos * half + u * V + i);
+				}
+				const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-			for (int p = 0; p < VP; ++p) {
-				unpack_unit(lo[b][p], x[p], (const T*)nullptr);
-				unpack_unit(hi[b][p], y[p], (const T*)nullptr);
-#pragma unroll
-				for (int i = 0; i < V; ++i) ss = fmaf(x[p][i], x[p][i], fmaf(y[p][i], y[p][i], ss));
+				for (int k = 0; k < 4; ++k) {
+					ac[p][i + k] = g0[i + k] * cc[k];
+					bs[p][i + k] = g1[i + k] * ss[k];
+					bc[p][i + k] = g1[i + k] * cc[k];
+					as[p][i + k] = g0[i + k] * ss[k];
+				}
 			}
-			for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-			if (h >= h1) continue;
-			if (!is_v) {
-				const T* gain = reinterpret_cast<const T*>(is_q ? a.q_gain : a.k_gain);
-				const float inv = gain ? 1.0f / sqrtf(ss / (float)a.hd + a.eps) : 1.0f;
+		}
+		uint8_t* dst = kind == 0 ? a.q_out + token * a.q_out_stride + (size_t)(from + grp) * head_bytes
+		                         : (kind == 1 ? a.kpool : a.vpool) + slab + (uint64_t)(from + grp - a.H - (kind == 2 ? a.KV : 0)) * a.blk * head_bytes;
+		const uint64_t dst_step = (uint64_t)groups * (kind == 0 ? head_bytes : (uint32_t)a.blk * head_bytes);
+		const bool stores = kind == 0 || page_ok;
+		for (int hb = from; hb < to; hb += kQnBatch * groups) {
+			uint4 lo[kQnBatch][VP], hi[kQnBatch][VP];
+#pragma unroll
+			for (int b = 0; b < kQnBatch; ++b)
 #pragma unroll
 				for (int p = 0; p < VP; ++p) {
-					if (!mine[p]) continue;
-					const int u = gl + p * a.lanes;
-					if (gain) {
-						float g0[V], g1[V];
-						unpack_unit(reinterpret_cast<const uint4*>(gain)[u], g0, (const T*)nullptr);
-						unpack_unit(reinterpret_cast<const uint4*>(gain)[u + half_units], g1, (const T*)nullptr);
+					lo[b][p] = hi[b][p] = make_uint4(0, 0, 0, 0);
+					if (mine[p] && hb + grp + b * groups < to) {
+						const uint4* src = reinterpret_cast<const uint4*>(row + (size_t)(hb + grp + b * groups) * head_bytes);
+						lo[b][p] = src[gl + p * a.lanes];
+						hi[b][p] = src[gl + p * a.lanes + half_units];
+					}
+				}
+#pragma unroll
+			for (int b = 0; b < kQnBatch; ++b) {
+				if (kind < 2) {
+					float x[VP][V], y[VP][V];
+					float ss = 0.0f;
+#pragma unroll
+					for (int p = 0; p < VP; ++p) {
+						unpack_unit(lo[b][p], x[p], (const T*)nullptr);
+						unpack_unit(hi[b][p], y[p], (const T*)nullptr);
+#pragma unroll
+						for (int i = 0; i < V; ++i) ss = fmaf(x[p][i], x[p][i], fmaf(y[p][i], y[p][i], ss));
+					}
+					float inv = 1.0f;
+					if (gain) { // the warp's
+						for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+						inv = rsqrtf(fmaf(ss, a.inv_hd, a.eps));
+					}
+#pragma unroll
+					for (int p = 0; p < VP; ++p) {
+						float r0[V], r1[V];
 #pragma unroll
 						for (int i = 0; i < V; ++i) {
-							x[p][i] = x[p][i] * inv * (a.gain_offset + g0[i]);
-							y[p][i] = y[p][i] * inv * (a.gain_offset + g1[i]);
+							r0[i] = inv * fmaf(x[p][i], ac[p][i], -(y[p][i] * bs[p][i]));
+							r1[i] = inv * fmaf(y[p][i], bc[p][i], x[p][i] * as[p][i]);
 						}
+						lo[b][p] = pack_unit(r0, (T*)nullptr);
+						hi[b][p] = pack_unit(r1, (T*)nullptr);
 					}
-					float r0[V], r1[V];
-#pragma unroll
-					for (int i = 0; i < V; ++i) {
-						r0[i] = x[p][i] * c[p][i] - y[p][i] * s[p][i];
-						r1[i] = y[p][i] * c[p][i] + x[p][i] * s[p][i];
-					}
-					lo[b][p] = pack_unit(r0, (T*)nullptr);
-					hi[b][p] = pack_unit(r1, (T*)nullptr);
 				}
-			}
-			uint8_t* dst;
-			if (is_q) {
-				dst = a.q_out + token * a.q_out_stride + (size_t)h * head_bytes;
-			} else {
-				if (!page_ok) continue;
-				const int kvh = h - a.H - (is_v ? a.KV : 0);
-				dst = (is_v ? a.vpool : a.kpool) + slab + (uint64_t)kvh * a.blk * head_bytes;
-			}
+				if (hb + grp + b * groups < to && stores) {
 #pragma unroll
-			for (int p = 0; p < VP; ++p) {
-				if (!mine[p]) continue;
-				reinterpret_cast<uint4*>(dst)[gl + p * a.lanes] = lo[b][p];
-				reinterpret_cast<uint4*>(dst)[gl + p * a.lanes + half_units] = hi[b][p];
+					for (int p = 0; p < VP; ++p) {
+						if (!mine[p]) continue;
+						reinterpret_cast<uint4*>(dst)[gl + p * a.lanes] = lo[b][p];
+						reinterpret_cast<uint4*>(dst)[gl + p * a.lanes + half_units] = hi[b][p];
+					}
+				}
+				dst += dst_step;
 			}
 		}
 	}

@@ -97,14 +97,13 @@ Error_t launch_qk_norm_rope(QkNormRopeArgs& a, int sms, cudaStream_t st)
 	a.lanes = 1;
 	while (a.lanes * vp < half_units) a.lanes <<= 1;
 	const int heads = a.H + 2 * a.KV;
-	// A group takes several heads of its token once there are groups enough to fill the SMs (2048 / 32
-	// warps each): cos and sin are then loaded once for them.
-	const u64 fill = (u64)sms * 2048 / (u64)a.lanes;
-	a.chunk = kQnBatch;
-	while (a.chunk < heads && (u64)a.n_tokens * ((heads + 2 * a.chunk - 1) / (2 * a.chunk)) >= fill) a.chunk *= 2;
-	if ((u64)a.n_tokens * ((heads + kQnBatch - 1) / kQnBatch) < fill) a.chunk = 1;
+	// A warp takes all heads of its token where there are tokens enough to fill the SMs (24 warps each); with
+	// fewer, as few heads as its groups hold at a time, so that a decode step's heads run side by side.
+	const int groups = kWarp / a.lanes;
+	a.chunk = heads;
+	while (a.chunk > groups && (u64)a.n_tokens * ((heads + a.chunk - 1) / a.chunk) < (u64)sms * 24) a.chunk = std::max(groups, (a.chunk + 1) / 2);
 	a.chunks = (heads + a.chunk - 1) / a.chunk;
-	const u64 ctas = ((u64)a.n_tokens * a.chunks * a.lanes + kQnThreads - 1) / kQnThreads;
+	const u64 ctas = ((u64)a.n_tokens * a.chunks + kQnThreads / kWarp - 1) / (kQnThreads / kWarp);
 	if (ctas > 0x7FFFFFFFull) return fail(ErrorUnsupported, "inf_qk_norm_rope: %u tokens of %d heads", a.n_tokens, heads);
 	return launch_pdl(vp == 2 ? k_qk_norm_rope_rows<T, 2> : k_qk_norm_rope_rows<T, 1>, dim3((unsigned)ctas), dim3(kQnThreads), 0, st, a);
 }
@@ -168,6 +167,7 @@ Error_t inf_qk_norm_rope(const InfPagedKv* kv, const InfQkNormRope* args, void* 
 	a.status = A.status;
 	a.eps = A.eps;
 	a.gain_offset = A.gain_offset;
+	a.inv_hd = (float)(1.0 / (double)hd);
 	a.n_pos = (int)A.n_pos;
 	a.n_tokens = A.n_tokens;
 	a.H = (int)A.n_heads;
