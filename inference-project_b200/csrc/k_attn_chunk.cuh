@@ -177,7 +177,8 @@ __device__ __forceinline__ void ac_prefix(const AttnChunkArgs& a, uint32_t* pre)
 }
 
 // A worker's run of the laid-out costs, walked item by item (every lane of the warp holds the same).
-template <int KT>
+// kOneTile: sequences of at most R rows only.
+template <int KT, bool kOneTile = false>
 struct AcRun {
 	uint32_t at, end, run; // position and end of the run, length of every run
 	int s, h, tile, tiles;
@@ -228,6 +229,11 @@ struct AcRun {
 		h = (int)(in / per_head);
 		uint32_t left = in % per_head;
 		item = at - left;
+		if (kOneTile) {
+			tile = 0;
+			tile_of(a);
+			return;
+		}
 		// the tile that holds `left`: 32 tiles at a time
 		for (tile = 0;; tile += kWarp) {
 			const int my = tile + lane;
@@ -273,19 +279,16 @@ struct AcRun {
 };
 
 // The record of an item that worker `w` begins and does not end (one lane calls it), or of none.
-template <int KT>
-__device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w, const AcRun<KT>* run)
+__device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w) { a.jobs[(size_t)w * kAcJobInts + kAcJobRows] = 0; }
+template <typename Run>
+__device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w, const Run& run)
 {
 	int* j = a.jobs + (size_t)w * kAcJobInts;
-	if (!run) {
-		j[kAcJobRows] = 0;
-		return;
-	}
-	j[kAcJobSeq] = run->q.row0;
-	j[kAcJobHead] = run->h;
-	j[kAcJobRow] = run->tile * a.R;
-	j[kAcJobRows] = run->rows();
-	j[kAcJobLast] = run->last_worker();
+	j[kAcJobSeq] = run.q.row0;
+	j[kAcJobHead] = run.h;
+	j[kAcJobRow] = run.tile * a.R;
+	j[kAcJobRows] = run.rows();
+	j[kAcJobLast] = run.last_worker();
 }
 
 // floats of one partial: R rows of O, each row's max and sum
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 	ac_prefix<kAfKT>(a, pre);
 	AcRun<kAfKT> run;
 	run.begin(a, pre, worker);
-	if (threadIdx.x == 0) ac_job<kAfKT>(a, worker, nullptr);
+	if (threadIdx.x == 0) ac_job(a, worker);
 	const float sl2 = a.scale * 1.4426950408889634f;
 	constexpr int V = Store<T>::kVec;
 	for (; !run.done(); run.next(a, pre)) {
@@ -557,7 +560,7 @@ __global__ void __launch_bounds__(kAfThreads) k_attn_chunk_f32(const AttnChunkAr
 				}
 			}
 		}
-		if (!whole && run.from() == 0 && threadIdx.x == 0) ac_job<kAfKT>(a, worker, &run);
+		if (!whole && run.from() == 0 && threadIdx.x == 0) ac_job(a, worker, run);
 	}
 }
 

@@ -64,34 +64,36 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 	ac_prefix<kCrKT>(a, pre); // ends with a barrier
 	const int worker = blockIdx.x * kCrWarps + warp;
 	if (worker >= a.workers) return;
-	if (lane == 0) ac_job<kCrKT>(a, worker, nullptr);
-	AcRun<kCrKT> run, load; // where the products and where the copies are
+	if (lane == 0) ac_job(a, worker);
+	AcRun<kCrKT, true> run, load; // where the products and where the copies are
 	run.begin(a, pre, worker);
 	load = run;
 
 	// ---- the copies, kStages tiles ahead
 	const uint64_t pol = policy_evict_first(); // read once
 	const int blk = a.blk;
-	int load_i = run.done() ? 0 : run.from(), issued = 0, stage_in = 0;
-	// page of the next tile to copy (-1: the tile of an item that sees nothing), read one copy ahead: a table
-	// entry takes as long to arrive as a tile's arithmetic
-	auto look = [&]() {
-		if (load.done()) return -1;
-		const int k0 = ac_tile_at(load.t, load_i) * kCrKT;
-		return k0 < load.t.hi ? a.table[(size_t)load.q.slot * a.pages_per_seq + k0 / blk] : -1;
+	int load_i = run.done() ? 0 : run.from(), load_to = run.done() ? 0 : run.to(), issued = 0, stage_in = 0;
+	// lane j holds the page of tile ids_i + j of the item being copied: a table entry takes as long to arrive as a
+	// tile's arithmetic, so they are read 32 at a time
+	int ids = 0, ids_i = 0;
+	auto refill = [&]() {
+		ids_i = load_i;
+		const int i = load_i + lane, k0 = load.done() ? 0 : ac_tile_at(load.t, i) * kCrKT;
+		ids = 0; // the tile of an item that sees nothing copies some page
+		if (!load.done() && i < load.to() && k0 < load.t.hi) {
+			ids = a.table[(size_t)load.q.slot * a.pages_per_seq + k0 / blk];
+			if (ids < 0 || ids >= a.n_pages) {
+				report_err(a.status, kDevKvRange);
+				ids = 0;
+			}
+		}
 	};
-	int ahead = look();
+	refill();
 	auto fetch = [&]() { // the whole warp; no-op behind the run's end
 		if (load.done()) return;
-		const int k0 = ac_tile_at(load.t, load_i) * kCrKT;
-		int page = ahead;
-		if (page < 0 || page >= a.n_pages) {
-			if (k0 < load.t.hi && lane == 0) report_err(a.status, kDevKvRange);
-			page = 0;
-		}
-		page = (int)__shfl_sync(0xFFFFFFFFu, page, 0);
+		const int page = __shfl_sync(0xFFFFFFFFu, ids, load_i - ids_i);
 		const int st = __shfl_sync(0xFFFFFFFFu, stage_in, 0), head_row = __shfl_sync(0xFFFFFFFFu, load.h * blk, 0);
-		const int group = __shfl_sync(0xFFFFFFFFu, (k0 & (blk - 1)) >> 3, 0); // blk is a power of two here
+		const int group = blk > kCrKT ? __shfl_sync(0xFFFFFFFFu, ((ac_tile_at(load.t, load_i) * kCrKT) & (blk - 1)) >> 3, 0) : 0;
 		uint8_t* dst = ring + (uint32_t)st * 2 * kTile;
 		if (elect_one()) {
 			mbar_arrive_expect_tx(&bars[st], 2 * kTile);
@@ -101,11 +103,15 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 		__syncwarp();
 		++issued;
 		if (++stage_in == kStages) stage_in = 0;
-		if (++load_i == load.to()) {
+		++load_i;
+		if (load_i == load_to) {
 			load.next(a, pre);
-			if (!load.done()) load_i = load.from();
+			load_i = load.done() ? 0 : load.from();
+			load_to = load.done() ? 0 : load.to();
+			refill();
+		} else if (load_i == ids_i + kWarp) {
+			refill();
 		}
-		ahead = look();
 	};
 	for (int i = 0; i < kStages; ++i) fetch();
 
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 				}
 			}
 		}
-		if (!whole && run.from() == 0 && lane == 0) ac_job<kCrKT>(a, worker, &run);
+		if (!whole && run.from() == 0 && lane == 0) ac_job(a, worker, run);
 	}
 	if (!ok && lane == 0) {
 		// never leave the CTA with copies in flight

@@ -455,11 +455,11 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 			const bool w = mbar_wait_cycles(&bars[bar], par, abort_flag, a.status);
 			return (bool)__all_sync(0xFFFFFFFFu, w);
 		};
-		if (warp == 0 && lane == 0) ac_job<kCtKT>(a, worker, nullptr);
+		if (warp == 0 && lane == 0) ac_job(a, worker);
 		while (ok && !run.done()) {
 			const int from = run.from(), to_tile = run.to();
 			const int valid = min(half_rows, run.rows() - sub * half_rows); // rows of this subtile
-			if (warp == 0 && lane == 0 && from == 0 && !run.whole()) ac_job<kCtKT>(a, worker, &run);
+			if (warp == 0 && lane == 0 && from == 0 && !run.whole()) ac_job(a, worker, run);
 			if (valid <= 0) {
 				ring.skip(2 * (to_tile - from), stages);
 				run.next(a, pre);
