@@ -103,6 +103,33 @@ __device__ __forceinline__ void unpack_unit(const uint4& u, float* out, const fl
 	out[2] = __uint_as_float(u.z); out[3] = __uint_as_float(u.w);
 }
 
+// ---- pairs of floats (one instruction each on sm_100) ----------------------------------
+__device__ __forceinline__ uint64_t f2(float lo, float hi)
+{
+	uint64_t r;
+	asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+	return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c)
+{
+	uint64_t r;
+	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+	return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b)
+{
+	uint64_t r;
+	asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b)
+{
+	uint64_t r;
+	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+
 // floats into one 16-byte unit, rounded to nearest even
 __device__ __forceinline__ uint4 pack_unit(const float* v, bf16*)
 {
