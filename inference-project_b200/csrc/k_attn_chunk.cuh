@@ -160,17 +160,24 @@ __device__ __forceinline__ void ac_prefix(const AttnChunkArgs& a, uint32_t* pre)
 	if (threadIdx.x == 0) pre[0] = 0;
 	__syncthreads();
 	if (warp == 0) {
-		uint32_t carry = 0;
+		// in 64 bits: sequences that name the same rows over and over (q_start going back and forth) cost more than
+		// the tokens allow, and such a call does nothing
+		uint64_t carry = 0;
 		for (int base = 0; base < a.n_seqs; base += kWarp) {
 			const int s = base + lane;
-			uint32_t v = s < a.n_seqs ? pre[s + 1] : 0u;
+			uint64_t v = s < a.n_seqs ? pre[s + 1] : 0u;
 #pragma unroll
 			for (int o = 1; o < 32; o <<= 1) {
-				const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, v, o);
+				const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, v, o);
 				if (lane >= o) v += y;
 			}
-			if (s < a.n_seqs) pre[s + 1] = carry + v;
+			if (s < a.n_seqs) pre[s + 1] = (uint32_t)(carry + v);
 			carry += __shfl_sync(0xFFFFFFFFu, v, 31);
+		}
+		if (carry > 0x7FFFFFFFull) {
+			__syncwarp();
+			for (int s = lane; s < a.n_seqs; s += kWarp) pre[s + 1] = 0;
+			if (report && lane == 0) report_err(a.status, kDevBadIndex);
 		}
 	}
 	__syncthreads();
@@ -235,7 +242,8 @@ struct AcRun {
 			return;
 		}
 		// the tile that holds `left`: 32 tiles at a time
-		for (tile = 0;; tile += kWarp) {
+		bool found = false;
+		for (tile = 0; tile < tiles && !found; tile += found ? 0 : kWarp) {
 			const int my = tile + lane;
 			const uint32_t c = my < tiles ? (uint32_t)ac_tile_cost<KT>(a, q, my) : 0u;
 			uint32_t x = c;
@@ -250,12 +258,14 @@ struct AcRun {
 				const int k = __ffs(hit) - 1;
 				item += __shfl_sync(0xFFFFFFFFu, x - c, k);
 				tile += k;
-				break;
+				found = true;
+			} else {
+				left -= all;
+				item += all;
 			}
-			left -= all;
-			item += all;
 		}
-		tile_of(a);
+		if (found) tile_of(a);
+		else end = at; // lengths that changed under the kernel: the run ends
 	}
 
 	__device__ __forceinline__ void next(const AttnChunkArgs& a, const uint32_t* pre)
@@ -268,7 +278,11 @@ struct AcRun {
 			if (++h == a.KV) {
 				h = 0;
 				do ++s;
-				while (pre[s + 1] == pre[s]);
+				while (s < a.n_seqs && pre[s + 1] == pre[s]);
+				if (s >= a.n_seqs) { // as above
+					end = at;
+					return;
+				}
 				q = ac_seq(a, s, false);
 				rows_ = q.n * a.G;
 				tiles = (rows_ + r_ - 1) / r_;

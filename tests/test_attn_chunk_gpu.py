@@ -246,3 +246,39 @@ def test_what_only_the_device_sees_is_reported(cuda, H, KV, hd, dtype):
     assert code == 11
     call, code = broken(lambda c: c.c.table.__setitem__((3, 2), c.c.n_pages))
     assert code == 11
+
+
+@pytest.mark.parametrize("H,KV,hd,dtype", [(8, 2, 128, "bf16"), (32, 1, 64, "bf16"), (4, 4, 48, "fp32")])
+def test_starts_that_go_back_and_forth(cuda, H, KV, hd, dtype):
+    """q_start 0, N, 0, N, ...: every second sequence is refused and the call reported; the rows hold what one
+    of the sequences that name them computes, and the call ends."""
+    torch = cuda
+    n, pairs = 40, 30
+    call = Call(torch, [(n, 60)] * pairs, H, KV, hd, dtype, extra_rows=0)
+    call.q_start.copy_(torch.tensor([n * (i % 2) for i in range(pairs + 1)], dtype=torch.int32))
+    call.run()
+    with pytest.raises(I.InfError) as e:
+        call.c.check()
+    assert e.value.code == 4
+    assert bool(call.out_all[:n].isfinite().all()) and bool((call.out_all[n:] == SENTINEL).all())
+
+
+def test_costs_beyond_32_bits_are_refused(cuda):
+    """The same with so many long sequences that the work would not fit 31 bits: reported, nothing written."""
+    torch = cuda
+    n_seqs, n, ctx = 4096, 8192, 1 << 20
+    c = Cache(torch, 1, ctx // 16, 1, 64, n_pages=4)
+    q = c.randn(n, 64 * 64)
+    out = torch.full_like(q, SENTINEL)
+    starts = torch.tensor([n * (i % 2) for i in range(n_seqs + 1)], dtype=torch.int32, device="cuda")
+    lens = torch.full((n_seqs,), ctx, dtype=torch.int32, device="cuda")
+    slot = torch.zeros(n_seqs, dtype=torch.int32, device="cuda")
+    nb = I.attn_chunk_scratch_bytes(c.kv, n_heads=64, n_tokens=n, n_seqs=n_seqs)
+    scratch = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    I.attn_chunk(c.kv, I.attn_chunk_args(
+        d_q=q.data_ptr(), d_out=out.data_ptr(), d_q_start=starts.data_ptr(), d_ctx_len=lens.data_ptr(), d_seq_slot=slot.data_ptr(),
+        n_seqs=n_seqs, n_tokens=n, n_heads=64, d_scratch=scratch.data_ptr(), scratch_bytes=nb, d_status=c.status.data_ptr()))
+    with pytest.raises(I.InfError) as e:
+        c.check()
+    assert e.value.code == 4
+    assert bool((out == SENTINEL).all())
