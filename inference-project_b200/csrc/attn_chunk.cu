@@ -2,6 +2,7 @@
 // and their number of workers from what the host knows (types, head layout, row counts at most), lays
 // out the scratch, and enqueues them.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -121,11 +122,13 @@ Error_t launch_tc(const AttnChunkArgs& a, const ChunkPass& p, cudaStream_t st)
 	INF_TRY(tensor_map_kv_groups(&v1, a.vpool, HD, blk, (u32)a.KV, (u32)a.n_pages, 1, blk / 8));
 	INF_TRY(allow_smem(k_attn_chunk_tc<HD>, 227 * 1024));
 	// the kernel's warpgroups trade registers within what it was launched with
-	static const int regs = [] {
+	static std::atomic<bool> regs_seen{false};
+	if (!regs_seen.load(std::memory_order_relaxed)) {
 		cudaFuncAttributes f;
-		return cudaFuncGetAttributes(&f, k_attn_chunk_tc<HD>) == cudaSuccess ? f.numRegs : 0;
-	}();
-	if (regs < kCtRegsLaunch) return fail(ErrorUnsupported, "inf_attn_chunk: built with %d registers a thread", regs);
+		INF_CUDA_TRY(cudaFuncGetAttributes(&f, k_attn_chunk_tc<HD>));
+		if (f.numRegs < kCtRegsLaunch) return fail(ErrorUnsupported, "inf_attn_chunk: built with %d registers a thread", f.numRegs);
+		regs_seen.store(true, std::memory_order_relaxed);
+	}
 	return launch_pdl(k_attn_chunk_tc<HD>, dim3((unsigned)p.workers), dim3(kCtThreads), p.smem, st, q, k8, k1, v8, v1, a);
 }
 

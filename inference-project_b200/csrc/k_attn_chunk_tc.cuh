@@ -33,15 +33,16 @@
 namespace inf {
 
 constexpr int kCtRows = 128; // rows of a subtile at most: floor(128 / G) tokens times G heads
-constexpr int kCtKT = 128;
+constexpr int kCtKT = 128;   // keys of a tile
 constexpr int kCtThreads = 384; // 3 warpgroups: subtile 0, subtile 1, copies and products
 // Registers: 168 a thread at launch; the softmax warpgroups, which hold a row of 128 scores, take of the third
-// one's share: 2 x 208 + 88 = 3 x 168.
-constexpr int kCtRegsLaunch = 168, kCtRegsSoftmax = 208, kCtRegsRest = 88;
+// one's share: 2 x 184 + 136 = 3 x 168, the split in which no role spills.
+constexpr int kCtRegsLaunch = 168, kCtRegsSoftmax = 184, kCtRegsRest = 136;
 static_assert(2 * kCtRegsSoftmax + kCtRegsRest <= 3 * kCtRegsLaunch, "register split");
 constexpr int kCtMaxStages = 12;
 constexpr uint32_t kCtAtom = 128 * 64 * 2; // one [128 x 64] bf16 SWIZZLE_128B block: 16 KB
-constexpr float kCtRescaleLog2 = 8.0f;
+constexpr float kCtRescaleLog2 = 8.0f;  // growth of a row's max that O is not rescaled for
+constexpr uint32_t kCtBarBytes = 304;
 
 enum CtBar : int {
 	kCtFull = 0,                          // [stages] tile in the ring
@@ -66,17 +67,17 @@ __host__ __device__ inline CtLayout ct_layout(int hd, int n_seqs)
 	L.tile = (uint32_t)(hd / 64) * kCtAtom;
 	L.q = 0;
 	L.ring = 2 * L.tile;
-	const uint32_t rest = 304 + 16 + (uint32_t)(n_seqs + 1) * 4;
+	const uint32_t rest = kCtBarBytes + 16 + (uint32_t)(n_seqs + 1) * 4;
 	const uint32_t room = 227 * 1024 - 1024 - rest - L.ring; // 1024: alignment of the swizzled blocks
 	L.stages = (int)(room / L.tile);
 	if (L.stages > kCtMaxStages) L.stages = kCtMaxStages;
 	L.bars = L.ring + (uint32_t)L.stages * L.tile;
-	L.flags = L.bars + 304;
+	L.flags = L.bars + kCtBarBytes;
 	L.pre = L.flags + 16;
 	L.total = 1024 + L.pre + (uint32_t)(n_seqs + 1) * 4;
 	return L;
 }
-static_assert(kCtBars * 8 <= 304, "barriers");
+static_assert(kCtBars * 8 <= kCtBarBytes, "barriers");
 
 // kind::f16 with A (rows x 16, two bf16 per column) in tensor memory
 __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
@@ -185,9 +186,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, worker = blockIdx.x;
 
 	if (threadIdx.x == 0) {
-		for (int i = 0; i < kCtBars; ++i) {
-			mbar_init(&bars[i], i >= kCtP && i < kCtO ? 4 : 1);
-		}
+		for (int i = 0; i < kCtBars; ++i) mbar_init(&bars[i], i >= kCtP && i < kCtO ? 4 : 1);
 		*abort_flag = 0;
 		mbar_fence_init();
 	}
@@ -201,224 +200,226 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 	ac_prefix<kCtKT>(a, pre); // ends with a barrier
 	tc_fence_after();
 	const uint32_t tmem = *tmem_slot;
-	AcRun<kCtKT> run;
-	run.begin(a, pre, worker);
 
 	if (warp >= 8) {
-	asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtRegsRest));
-	if (warp == 8 || warp == 10) {
-		// ---------------- TMA producers: K tiles (warp 8) and V tiles (warp 10), every other entry of the ring
-		const bool is_v = warp == 10;
-		const CUtensorMap* tm8 = is_v ? &tm_v8 : &tm_k8;
-		const CUtensorMap* tm1 = is_v ? &tm_v1 : &tm_k1;
-		const uint64_t pol = policy_evict_normal();
-		const int blk = a.blk, pages = kCtKT / blk;
-		CtRing r;
-		if (is_v) r.next(stages);
-		uint32_t entry = is_v ? 1u : 0u; // entries of the ring before this one
-		bool ok = true;
-		for (; ok && !run.done(); run.next(a, pre)) {
-			const int* bt = a.table + (size_t)run.q.slot * a.pages_per_seq;
-			const int hi = run.t.hi, lo = run.t.lo, sinks = min(a.n_sink, hi);
-			// lane p holds page p of the tile; pages that no row sees stay out.  The next tile's ids are read
-			// before this one's stage is waited for.
-			auto sees = [&](int i) {
-				const int kp = ac_tile_at(run.t, i) * kCtKT + lane * blk;
-				return lane < pages && kp < hi && (kp + blk > lo || kp < sinks);
-			};
-			auto look = [&](int i) { return sees(i) ? bt[ac_tile_at(run.t, i) * pages + lane] : 0; };
-			int ahead = look(run.from());
-			for (int i = run.from(); ok && i < run.to(); ++i) {
-				const bool seen = sees(i);
-				int page = ahead;
-				ahead = i + 1 < run.to() ? look(i + 1) : 0;
-				if (seen && (page < 0 || page >= a.n_pages)) {
-					report_err(a.status, kDevKvRange);
-					page = 0;
-				}
-				const unsigned mask = __ballot_sync(0xFFFFFFFFu, seen);
-				const int page0 = __shfl_sync(0xFFFFFFFFu, page, 0);
-				const bool one_box = mask == (1u << pages) - 1u && __all_sync(0xFFFFFFFFu, lane >= pages || page == page0 + lane);
-				const uint32_t bytes = (uint32_t)__popc(mask) * (uint32_t)blk * HD * 2;
-				if (entry >= (uint32_t)stages) {
-					const bool w = mbar_wait_cycles<64>(&bars[kCtEmpty + r.stage], r.phase ^ 1u, abort_flag, a.status);
-					ok = __all_sync(0xFFFFFFFFu, w);
-					if (!ok) break;
-				}
-				const uint32_t stage = uniform((uint32_t)r.stage);
-				uint8_t* dst = ring_s + stage * kTile;
-				uint64_t* full = &bars[kCtFull + stage];
-				const int head_row = (int)uniform((uint32_t)(run.h * blk));
-				if (elect_one()) {
-					if (bytes) mbar_arrive_expect_tx(full, bytes);
-					else mbar_arrive(full);
-				}
-				__syncwarp();
-				if (one_box) {
-					if (elect_one()) tma_load_5d(dst, tm8, 0, head_row, 0, 0, page0, full, pol);
-				} else {
-#pragma unroll
-					for (int p = 0; p < kCtKT / 16; ++p) {
-						const int id = __shfl_sync(0xFFFFFFFFu, page, p);
-						if (((mask >> p) & 1u) && elect_one()) tma_load_5d(dst + (uint32_t)(p * blk) * HD * 2, tm1, 0, head_row, 0, 0, id, full, pol);
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtRegsRest));
+		AcRun<kCtKT> run; // begun behind setmaxnreg: state held across it spills
+		run.begin(a, pre, worker);
+		if (warp == 8 || warp == 10) {
+			// ---------------- TMA producers: K tiles (warp 8) and V tiles (warp 10), every other entry of the ring
+			const bool is_v = warp == 10;
+			const CUtensorMap* tm8 = is_v ? &tm_v8 : &tm_k8;
+			const CUtensorMap* tm1 = is_v ? &tm_v1 : &tm_k1;
+			const uint64_t pol = policy_evict_normal();
+			const int blk = a.blk, pages = kCtKT / blk;
+			CtRing r;
+			if (is_v) r.next(stages);
+			uint32_t entry = is_v ? 1u : 0u; // entries of the ring before this one
+			bool ok = true;
+			for (; ok && !run.done(); run.next(a, pre)) {
+				const int* bt = a.table + (size_t)run.q.slot * a.pages_per_seq;
+				const int hi = run.t.hi, lo = run.t.lo, sinks = min(a.n_sink, hi);
+				// lane p holds page p of the tile; pages that no row sees stay out.  The next tile's ids are read
+				// before this one's stage is waited for.
+				auto sees = [&](int i) {
+					const int kp = ac_tile_at(run.t, i) * kCtKT + lane * blk;
+					return lane < pages && kp < hi && (kp + blk > lo || kp < sinks);
+				};
+				auto look = [&](int i) { return sees(i) ? bt[ac_tile_at(run.t, i) * pages + lane] : 0; };
+				int ahead = look(run.from());
+				for (int i = run.from(); ok && i < run.to(); ++i) {
+					const bool seen = sees(i);
+					int page = ahead;
+					ahead = i + 1 < run.to() ? look(i + 1) : 0;
+					if (seen && (page < 0 || page >= a.n_pages)) {
+						report_err(a.status, kDevKvRange);
+						page = 0;
 					}
+					const unsigned mask = __ballot_sync(0xFFFFFFFFu, seen);
+					const int page0 = __shfl_sync(0xFFFFFFFFu, page, 0);
+					const bool one_box = mask == (1u << pages) - 1u && __all_sync(0xFFFFFFFFu, lane >= pages || page == page0 + lane);
+					const uint32_t bytes = (uint32_t)__popc(mask) * (uint32_t)blk * HD * 2;
+					if (entry >= (uint32_t)stages) {
+						const bool w = mbar_wait_cycles<64>(&bars[kCtEmpty + r.stage], r.phase ^ 1u, abort_flag, a.status);
+						ok = __all_sync(0xFFFFFFFFu, w);
+						if (!ok) break;
+					}
+					const uint32_t stage = uniform((uint32_t)r.stage);
+					uint8_t* dst = ring_s + stage * kTile;
+					uint64_t* full = &bars[kCtFull + stage];
+					const int head_row = (int)uniform((uint32_t)(run.h * blk));
+					if (elect_one()) {
+						if (bytes) mbar_arrive_expect_tx(full, bytes);
+						else mbar_arrive(full);
+					}
+					__syncwarp();
+					if (one_box) {
+						if (elect_one()) tma_load_5d(dst, tm8, 0, head_row, 0, 0, page0, full, pol);
+					} else {
+#pragma unroll
+						for (int p = 0; p < kCtKT / 16; ++p) {
+							const int id = __shfl_sync(0xFFFFFFFFu, page, p);
+							if (((mask >> p) & 1u) && elect_one()) tma_load_5d(dst + (uint32_t)(p * blk) * HD * 2, tm1, 0, head_row, 0, 0, id, full, pol);
+						}
+					}
+					entry += 2;
+					r.skip(2, stages);
 				}
-				entry += 2;
-				r.skip(2, stages);
 			}
-		}
-		if (!ok) {
-			// never leave the CTA with copies in flight: this producer's last entries
-			__syncwarp();
-			CtRing back;
-			if (is_v) back.next(stages);
-			for (uint32_t i = is_v ? 1u : 0u; i < entry; i += 2, back.skip(2, stages)) {
-				if (i + (uint32_t)stages < entry) continue;
-				const uint64_t t0 = global_timer_ns();
-				while (!mbar_try_wait(&bars[kCtFull + back.stage], back.phase))
-					if (global_timer_ns() - t0 > kWaitLimitNs) break;
-			}
-		}
-	} else if (warp == 9) {
-		// ---------------- product issuer: the warp runs the pipeline converged, one elected lane issues
-		constexpr uint32_t idesc_s = umma_idesc_bf16(128, kCtKT);
-		constexpr uint32_t idesc_o = umma_idesc_bf16(128, HD) | (1u << 16); // B (V) MN-major
-		const uint32_t qa = smem_u32(q_s), ra = smem_u32(ring_s), tm = uniform(tmem);
-		CtRing r;
-		uint32_t q_par[2] = {0, 0}, p_par[2] = {0, 0};
-		auto wait = [&](int bar, uint32_t par) {
-			const bool w = mbar_wait_cycles(&bars[bar], par, abort_flag, a.status);
-			return (bool)__all_sync(0xFFFFFFFFu, w);
-		};
-		auto mma_s = [&](int sub, uint32_t stage) { // by the elected lane
-			const uint64_t da = umma_desc_sw128(qa + (uint32_t)sub * kTile);
-			const uint64_t db = umma_desc_sw128_lbo(ra + stage * kTile, 16, kGroup);
-#pragma unroll
-			for (int k = 0; k < HD / 16; ++k)
-				umma_bf16(tm + (uint32_t)sub * kCtKT, da + (uint32_t)((k >> 2) * (kCtAtom / 16) + (k & 3) * 2),
-				          db + (uint32_t)((k >> 2) * 64 + (k & 3) * 2), idesc_s, k > 0 ? 1u : 0u);
-			umma_commit(&bars[kCtS + sub]);
-		};
-		auto mma_pv = [&](int sub, uint32_t stage, uint32_t acc) {
-			const uint64_t dv = umma_desc_sw128_lbo(ra + stage * kTile, 1024, kGroup);
-			const uint32_t pa = tm + (uint32_t)sub * kCtKT, od = tm + 2 * kCtKT + (uint32_t)(sub * HD);
-#pragma unroll
-			for (int k = 0; k < kCtKT / 16; ++k)
-				umma_bf16_ts(od, pa + (uint32_t)k * 8, dv + (uint32_t)(k * 2 * kGroup / 16), idesc_o, k > 0 ? 1u : acc);
-		};
-		bool ok = true, busy = !run.done();
-		int n = busy ? run.to() - run.from() : 0, subs = busy && run.rows() > (a.R >> 1) ? 2 : 1;
-		while (ok && busy) {
-			// S of the first tile
-			uint32_t ks = uniform((uint32_t)r.stage);
-			ok = wait(kCtFull + (int)ks, r.phase);
-#pragma unroll
-			for (int sub = 0; sub < 2; ++sub) {
-				if (!ok || sub >= subs) break;
-				ok = wait(kCtQ + sub, q_par[sub]);
-				if (!ok) break;
-				q_par[sub] ^= 1u;
-				tc_fence_after();
-				if (elect_one()) {
-					mma_s(sub, ks);
-					if (n == 1) umma_commit(&bars[kCtQFree + sub]);
-					if (sub == subs - 1) umma_commit(&bars[kCtEmpty + ks]);
-				}
+			if (!ok) {
+				// never leave the CTA with copies in flight: this producer's last entries
 				__syncwarp();
-			}
-			if (!ok) break;
-			r.next(stages);
-			// the next item, found while the softmax warps work
-			run.next(a, pre);
-			busy = !run.done();
-			const int next_n = busy ? run.to() - run.from() : 0, next_subs = busy && run.rows() > (a.R >> 1) ? 2 : 1;
-			for (int j = 0; ok && j < n; ++j) {
-				// V of this tile and K of the next are waited for ahead of P, so that nothing but the issue
-				// stands between P's second half and the next S
-				const uint32_t vs = uniform((uint32_t)r.stage);
-				ok = wait(kCtFull + (int)vs, r.phase);
-				if (!ok) break;
-				r.next(stages);
-				const bool more = j + 1 < n, last_s = j + 2 == n;
-				if (more) {
-					ks = uniform((uint32_t)r.stage);
-					ok = wait(kCtFull + (int)ks, r.phase);
-					if (!ok) break;
-					r.next(stages);
+				CtRing back;
+				if (is_v) back.next(stages);
+				for (uint32_t i = is_v ? 1u : 0u; i < entry; i += 2, back.skip(2, stages)) {
+					if (i + (uint32_t)stages < entry) continue;
+					const uint64_t t0 = global_timer_ns();
+					while (!mbar_try_wait(&bars[kCtFull + back.stage], back.phase))
+						if (global_timer_ns() - t0 > kWaitLimitNs) break;
 				}
-				const uint32_t acc = j > 0 ? 1u : 0u;
+			}
+		} else if (warp == 9) {
+			// ---------------- product issuer: the warp runs the pipeline converged, one elected lane issues
+			constexpr uint32_t idesc_s = umma_idesc_bf16(128, kCtKT);
+			constexpr uint32_t idesc_o = umma_idesc_bf16(128, HD) | (1u << 16); // B (V) MN-major
+			const uint32_t qa = smem_u32(q_s), ra = smem_u32(ring_s), tm = uniform(tmem);
+			CtRing r;
+			uint32_t q_par[2] = {0, 0}, p_par[2] = {0, 0};
+			auto wait = [&](int bar, uint32_t par) {
+				const bool w = mbar_wait_cycles(&bars[bar], par, abort_flag, a.status);
+				return (bool)__all_sync(0xFFFFFFFFu, w);
+			};
+			auto mma_s = [&](int sub, uint32_t stage) { // by the elected lane
+				const uint64_t da = umma_desc_sw128(qa + (uint32_t)sub * kTile);
+				const uint64_t db = umma_desc_sw128_lbo(ra + stage * kTile, 16, kGroup);
+#pragma unroll
+				for (int k = 0; k < HD / 16; ++k)
+					umma_bf16(tm + (uint32_t)sub * kCtKT, da + (uint32_t)((k >> 2) * (kCtAtom / 16) + (k & 3) * 2),
+					          db + (uint32_t)((k >> 2) * 64 + (k & 3) * 2), idesc_s, k > 0 ? 1u : 0u);
+				umma_commit(&bars[kCtS + sub]);
+			};
+			auto mma_pv = [&](int sub, uint32_t stage, uint32_t acc) {
+				const uint64_t dv = umma_desc_sw128_lbo(ra + stage * kTile, 1024, kGroup);
+				const uint32_t pa = tm + (uint32_t)sub * kCtKT, od = tm + 2 * kCtKT + (uint32_t)(sub * HD);
+#pragma unroll
+				for (int k = 0; k < kCtKT / 16; ++k)
+					umma_bf16_ts(od, pa + (uint32_t)k * 8, dv + (uint32_t)(k * 2 * kGroup / 16), idesc_o, k > 0 ? 1u : acc);
+			};
+			bool ok = true, busy = !run.done();
+			int n = busy ? run.to() - run.from() : 0, subs = busy && run.rows() > (a.R >> 1) ? 2 : 1;
+			while (ok && busy) {
+				// S of the first tile
+				uint32_t ks = uniform((uint32_t)r.stage);
+				ok = wait(kCtFull + (int)ks, r.phase);
 #pragma unroll
 				for (int sub = 0; sub < 2; ++sub) {
 					if (!ok || sub >= subs) break;
-					ok = wait(kCtP + sub, p_par[sub]);
+					ok = wait(kCtQ + sub, q_par[sub]);
 					if (!ok) break;
-					p_par[sub] ^= 1u;
+					q_par[sub] ^= 1u;
 					tc_fence_after();
 					if (elect_one()) {
-						mma_pv(sub, vs, acc);
-						if (more) {
-							mma_s(sub, ks);
-							if (last_s) umma_commit(&bars[kCtQFree + sub]);
-						} else {
-							umma_commit(&bars[kCtO + sub]);
-						}
-						if (sub == subs - 1) {
-							umma_commit(&bars[kCtEmpty + vs]);
-							if (more) umma_commit(&bars[kCtEmpty + ks]);
-						}
+						mma_s(sub, ks);
+						if (n == 1) umma_commit(&bars[kCtQFree + sub]);
+						if (sub == subs - 1) umma_commit(&bars[kCtEmpty + ks]);
 					}
 					__syncwarp();
 				}
-			}
-			n = next_n;
-			subs = next_subs;
-		}
-		// every product is done before tensor memory is freed, whatever ended the loop
-		if (elect_one()) umma_commit(&bars[kCtDrain]);
-		__syncwarp();
-		const long long t0 = clock64();
-		while (!mbar_try_wait(&bars[kCtDrain], 0))
-			if (clock64() - t0 > kWaitLimitCycles) break;
-		__syncwarp();
-	} else {
-		// ---------------- TMA producer of Q: both subtiles of the next item while the last one finishes
-		const uint32_t bytes = (uint32_t)(a.R >> 1) * HD * 2;
-		const int toks = a.group.div(a.R >> 1); // tokens of a subtile
-		const uint64_t pol = policy_evict_first();
-		uint32_t uses[2] = {0, 0};
-		bool ok = true;
-		for (; ok && !run.done(); run.next(a, pre)) {
-			const int subs = run.rows() > (a.R >> 1) ? 2 : 1;
-			const int head = (int)uniform((uint32_t)(run.h * a.G)), tok = (int)uniform((uint32_t)(run.q.row0 + run.tile * 2 * toks));
-#pragma unroll
-			for (int sub = 0; sub < 2; ++sub) {
-				if (!ok || sub >= subs) break;
-				if (uses[sub] > 0) {
-					const bool w = mbar_wait_cycles<500>(&bars[kCtQFree + sub], (uses[sub] - 1) & 1u, abort_flag, a.status);
-					ok = __all_sync(0xFFFFFFFFu, w);
+				if (!ok) break;
+				r.next(stages);
+				// the next item, found while the softmax warps work
+				run.next(a, pre);
+				busy = !run.done();
+				const int next_n = busy ? run.to() - run.from() : 0, next_subs = busy && run.rows() > (a.R >> 1) ? 2 : 1;
+				for (int j = 0; ok && j < n; ++j) {
+					// V of this tile and K of the next are waited for ahead of P, so that nothing but the issue
+					// stands between P's second half and the next S
+					const uint32_t vs = uniform((uint32_t)r.stage);
+					ok = wait(kCtFull + (int)vs, r.phase);
 					if (!ok) break;
-				}
-				if (elect_one()) {
-					mbar_arrive_expect_tx(&bars[kCtQ + sub], bytes);
+					r.next(stages);
+					const bool more = j + 1 < n, last_s = j + 2 == n;
+					if (more) {
+						ks = uniform((uint32_t)r.stage);
+						ok = wait(kCtFull + (int)ks, r.phase);
+						if (!ok) break;
+						r.next(stages);
+					}
+					const uint32_t acc = j > 0 ? 1u : 0u;
 #pragma unroll
-					for (int h = 0; h < kHalves; ++h)
-						tma_load_3d(q_s + (uint32_t)sub * kTile + h * kCtAtom, &tm_q, h * 64, head, tok + sub * toks, &bars[kCtQ + sub], pol);
+					for (int sub = 0; sub < 2; ++sub) {
+						if (!ok || sub >= subs) break;
+						ok = wait(kCtP + sub, p_par[sub]);
+						if (!ok) break;
+						p_par[sub] ^= 1u;
+						tc_fence_after();
+						if (elect_one()) {
+							mma_pv(sub, vs, acc);
+							if (more) {
+								mma_s(sub, ks);
+								if (last_s) umma_commit(&bars[kCtQFree + sub]);
+							} else {
+								umma_commit(&bars[kCtO + sub]);
+							}
+							if (sub == subs - 1) {
+								umma_commit(&bars[kCtEmpty + vs]);
+								if (more) umma_commit(&bars[kCtEmpty + ks]);
+							}
+						}
+						__syncwarp();
+					}
 				}
-				__syncwarp();
-				++uses[sub];
+				n = next_n;
+				subs = next_subs;
+			}
+			// every product is done before tensor memory is freed, whatever ended the loop
+			if (elect_one()) umma_commit(&bars[kCtDrain]);
+			__syncwarp();
+			const long long t0 = clock64();
+			while (!mbar_try_wait(&bars[kCtDrain], 0))
+				if (clock64() - t0 > kWaitLimitCycles) break;
+			__syncwarp();
+		} else {
+			// ---------------- TMA producer of Q: both subtiles of the next item while the last one finishes
+			const uint32_t bytes = (uint32_t)(a.R >> 1) * HD * 2;
+			const int toks = a.group.div(a.R >> 1); // tokens of a subtile
+			const uint64_t pol = policy_evict_first();
+			uint32_t uses[2] = {0, 0};
+			bool ok = true;
+			for (; ok && !run.done(); run.next(a, pre)) {
+				const int subs = run.rows() > (a.R >> 1) ? 2 : 1;
+				const int head = (int)uniform((uint32_t)(run.h * a.G)), tok = (int)uniform((uint32_t)(run.q.row0 + run.tile * 2 * toks));
+#pragma unroll
+				for (int sub = 0; sub < 2; ++sub) {
+					if (!ok || sub >= subs) break;
+					if (uses[sub] > 0) {
+						const bool w = mbar_wait_cycles<500>(&bars[kCtQFree + sub], (uses[sub] - 1) & 1u, abort_flag, a.status);
+						ok = __all_sync(0xFFFFFFFFu, w);
+						if (!ok) break;
+					}
+					if (elect_one()) {
+						mbar_arrive_expect_tx(&bars[kCtQ + sub], bytes);
+#pragma unroll
+						for (int h = 0; h < kHalves; ++h)
+							tma_load_3d(q_s + (uint32_t)sub * kTile + h * kCtAtom, &tm_q, h * 64, head, tok + sub * toks, &bars[kCtQ + sub], pol);
+					}
+					__syncwarp();
+					++uses[sub];
+				}
+			}
+			if (!ok) {
+				for (int sub = 0; sub < 2; ++sub) { // copies in flight
+					if (uses[sub] == 0) continue;
+					const long long t0 = clock64();
+					while (!mbar_try_wait(&bars[kCtQ + sub], (uses[sub] - 1) & 1u))
+						if (clock64() - t0 > kWaitLimitCycles) break;
+				}
 			}
 		}
-		if (!ok) {
-			for (int sub = 0; sub < 2; ++sub) { // copies in flight
-				if (uses[sub] == 0) continue;
-				const long long t0 = clock64();
-				while (!mbar_try_wait(&bars[kCtQ + sub], (uses[sub] - 1) & 1u))
-					if (clock64() - t0 > kWaitLimitCycles) break;
-			}
-		}
-	}
 	} else {
 		asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kCtRegsSoftmax));
+		AcRun<kCtKT> run;
+		run.begin(a, pre, worker);
 		// ---------------- softmax: subtile `sub`, a thread per row
 		const int sub = warp >> 2, quarter = warp & 3;
 		const int r = quarter * 32 + lane, half_rows = a.R >> 1;
@@ -560,8 +561,8 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 				tmem_ld_32(to + (uint32_t)c + 32, o[1]);
 				tmem_ld_wait(o[0]);
 				tmem_ld_wait(o[1]);
-				if (r >= valid) continue;
-				if (whole) {
+				if (r >= valid) {
+				} else if (whole) {
 #pragma unroll
 					for (int u = 0; u < 8; ++u) {
 						const float* x = &o[u >> 2][(u & 3) * 8];
@@ -575,6 +576,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 						reinterpret_cast<float4*>(part)[(size_t)(c / 4 + u) * a.R + pr] = make_float4(x[0], x[1], x[2], x[3]);
 					}
 				}
+				__syncwarp(); // together again for the next tcgen05.ld
 			}
 			if (!whole && r < valid) {
 				part[(size_t)a.R * HD + pr] = m;

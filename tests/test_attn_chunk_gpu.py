@@ -14,11 +14,12 @@ class Call:
     """Buffers of one call; the rows behind the last sequence hold a sentinel."""
 
     def __init__(self, torch, seqs, H, KV, hd, dtype="bf16", blk=16, window=0, sinks=0, scale=0.0, seed=0, extra_rows=3,
-                 pad=0, layers=1, layer=0, q_scale=1.5, max_new=None, slots=None, evict=True):
+                 pad=0, layers=1, layer=0, q_scale=1.5, max_new=None, slots=None, evict=True, spare=3):
         n = len(seqs)
         longest = max(max(ctx for _, ctx in seqs), 1)
         self.slots = slots or list(range(n))
-        self.c = c = Cache(torch, max(self.slots) + 1, -(-longest // blk) + 1, KV, hd, blk, dtype, layers, seed=seed)
+        self.c = c = Cache(torch, max(self.slots) + 1, -(-longest // blk) + 1, KV, hd, blk, dtype, layers, spare=spare,
+                           seed=seed)
         for (rows, ctx), s in zip(seqs, self.slots):
             keep = visible(rows, ctx, window, sinks) if evict else list(range(ctx))
             if rows:
@@ -282,3 +283,10 @@ def test_costs_beyond_32_bits_are_refused(cuda):
         c.check()
     assert e.value.code == 4
     assert bool((out == SENTINEL).all())
+
+
+@pytest.mark.parametrize("H,KV,hd,dtype,spare", [(32, 8, 128, "bf16", 270_000), (8, 8, 64, "fp32", 270_000)])
+def test_pages_past_4_gb(cuda, H, KV, hd, dtype, spare):
+    """Pools of 8.8 GB: half of the pages that a random draw takes lie beyond 32-bit byte offsets."""
+    call = check(cuda, [(1, 300), (3, 40), (60, 200)], H, KV, hd, dtype, spare=spare, seed=6)
+    assert int(call.c.table.max()) * KV * 16 * hd * call.c.k.element_size() > 1 << 32

@@ -18,9 +18,9 @@ def tables(torch, n_pos, hd, theta=500000.0):
 
 class Call:
     def __init__(self, torch, tokens, H, KV, hd, dtype="bf16", blk=16, gains=(True, True), offset=0.0, eps=1e-6, pad=0,
-                 layers=1, layer=0, in_place=False, slots=4, pps=8, seed=0, theta=500000.0):
+                 layers=1, layer=0, in_place=False, slots=4, pps=8, seed=0, theta=500000.0, spare=3):
         self.torch, self.H, self.KV, self.hd, self.layer = torch, H, KV, hd, layer
-        self.c = c = Cache(torch, slots, pps, KV, hd, blk, dtype, layers, seed=seed)
+        self.c = c = Cache(torch, slots, pps, KV, hd, blk, dtype, layers, spare=spare, seed=seed)
         self.tokens = tokens  # (slot, position)
         for s, p in tokens:
             if 0 <= s < slots and 0 <= p < pps * blk and int(c.table[s, p // blk]) < 0:
@@ -120,6 +120,13 @@ def test_strides_in_place_layers_and_page_sizes(cuda):
         call = Call(cuda, BATCH, 8, 2, 128, **kw)
         call.run()
         call.verify()
+
+
+def test_pages_past_4_gb(cuda):
+    call = Call(cuda, BATCH, 8, 8, 128, spare=270_000, seed=1)
+    assert int(call.c.table.max()) * 8 * 16 * 128 * 2 > 1 << 32
+    call.run()
+    call.verify()
 
 
 def test_rows_of_zeros_and_large_values(cuda):
