@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 				const int next_n = busy ? run.to() - run.from() : 0, next_subs = busy && run.rows() > (a.R >> 1) ? 2 : 1;
 				for (int j = 0; ok && j < n; ++j) {
 					// V of this tile and K of the next are waited for ahead of P, so that nothing but the issue
-					// stands between P's second half and the next S
+					// stands between P and the next S
 					const uint32_t vs = uniform((uint32_t)r.stage);
 					ok = wait(kCtFull + (int)vs, r.phase);
 					if (!ok) break;
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 				m = mn;
 				const float mu = m == -INFINITY ? 0.0f : m; // nothing seen yet: 2^(-inf) = 0
 				const uint64_t mux2 = f2(-mu, -mu);
-				// V rows that no row of the item sees become zeros, ahead of P's first half
+				// V rows that no row of the item sees become zeros, ahead of P
 				if (__builtin_expect(ragged, 0)) {
 					ok = wait(kCtFull + vstage, vphase);
 					if (!ok) break;
