@@ -21,7 +21,7 @@ u64 up256(u64 n) { return (n + 255) & ~255ull; }
 struct ChunkPass {
 	enum Kind { F32, Rows, TC } kind;
 	int rows_min, rows_max;
-	int workers, min_run;
+	int workers, min_run, item_cost;
 	int R;               // row tile
 	size_t smem;
 	u64 part_off, jobs_off;
@@ -33,12 +33,12 @@ struct ChunkPlan {
 	u64 scratch;
 };
 
-// Items times key tiles at most.
-u64 units_max(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, u32 R, u32 KT)
+// Items times their cost at most.
+u64 units_max(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, u32 R, u32 KT, u32 item_cost)
 {
 	const u64 G = n_heads / kv->n_kv_heads;
 	const u64 tiles = (u64)n_tokens * G / R + std::min(n_seqs, n_tokens);
-	return tiles * kv->n_kv_heads * (((u64)kv->pages_per_seq * kv->kv_block + KT - 1) / KT + 1);
+	return tiles * kv->n_kv_heads * (((u64)kv->pages_per_seq * kv->kv_block + KT - 1) / KT + 1 + item_cost);
 }
 
 Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, ChunkPlan* P)
@@ -87,10 +87,11 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 		t.rows_min = G <= (u32)kCrRows ? kCrRows : 0;
 		t.rows_max = 0x7FFFFFFF;
 		t.R = (int)(2 * (kCtRows / G) * G); // whole tokens in each half
-		t.min_run = 2;
+		t.item_cost = kCtItemCost;
+		t.min_run = 2 + kCtItemCost;
 		t.smem = ct_layout((int)kv->head_dim, (int)n_seqs).total;
 		t.workers = sms;
-		return add(t, units_max(kv, n_heads, n_tokens, n_seqs, (u32)t.R, kCtKT));
+		return add(t, units_max(kv, n_heads, n_tokens, n_seqs, (u32)t.R, kCtKT, kCtItemCost));
 	}
 	ChunkPass f = {};
 	f.kind = ChunkPass::F32;
@@ -99,7 +100,7 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 	f.min_run = 2;
 	f.smem = attn_chunk_f32_smem((int)kv->head_dim, (int)n_seqs);
 	f.workers = sms * (int)std::max<u64>(1, std::min<u64>(8, (200u << 10) / f.smem));
-	return add(f, units_max(kv, n_heads, n_tokens, n_seqs, kAfR, kAfKT));
+	return add(f, units_max(kv, n_heads, n_tokens, n_seqs, kAfR, kAfKT, 0));
 }
 
 template <typename T>
@@ -215,6 +216,7 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 		b.R = p.R;
 		b.workers = p.workers;
 		b.min_run = p.min_run;
+		b.item_cost = p.item_cost;
 		b.part = (float*)((uint8_t*)A.scratch + p.part_off);
 		b.jobs = (int*)((uint8_t*)A.scratch + p.jobs_off);
 		return b;

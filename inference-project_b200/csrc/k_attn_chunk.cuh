@@ -5,10 +5,10 @@
 // An item is (sequence, KV head, row tile): the rows of a sequence and KV head are its new tokens times
 // the G query heads of the group, row r = token * G + head, R of them to an item, so K and V are read
 // once per tile for the whole group.  The keys an item sees come in key tiles of KT positions: those of
-// the sinks, then those from the window's start to the last row's position; their number is the item's
-// cost.  All costs laid end to end (sequence, head, tile) are cut into equal runs, one per worker: a
-// worker may begin inside one item and end inside another, and every worker has the same number of key
-// tiles whatever the lengths are.  Where a cut falls inside an item each worker stores its share
+// the sinks, then those from the window's start to the last row's position; their number, and what an
+// item costs beside them, is its cost.  All costs laid end to end (sequence, head, tile) are cut into
+// equal runs, one per worker: a worker may begin inside one item and end inside another, and every worker
+// has the same work whatever the lengths are.  Where a cut falls inside an item each worker stores its share
 // (O, max, sum), and k_attn_chunk_combine joins them in the workers' order, so a result does not depend
 // on which worker finishes first.  Every warp finds its run from the lengths on the device: the host
 // needs none of them, and a captured launch follows new lengths.
@@ -58,7 +58,8 @@ struct AttnChunkArgs {
 	int rows_min, rows_max;
 	int R;                         // rows of an item
 	int workers;
-	int min_run;                   // key tiles of a worker at least
+	int min_run;                   // cost of a worker's run at least
+	int item_cost;                 // what an item costs beside its key tiles, in key tiles
 	int late_wait;                 // this kernel may run beside the one before it and waits for it at its end
 	float* part;                   // [2 * workers][hd + 2][R] partial O (unnormalised), max (log2 units), sum
 	int* jobs;                     // [workers][kAcJobInts]: the item that a worker begins and others end
@@ -127,7 +128,7 @@ __device__ __forceinline__ bool ac_sees(const AttnChunkArgs& a, int p, int k)
 template <int KT>
 __device__ __forceinline__ int ac_tile_cost(const AttnChunkArgs& a, const AcSeq& q, int tile)
 {
-	return ac_tiles<KT>(a, q, tile * a.R, min((tile + 1) * a.R, q.n * a.G)).cost;
+	return ac_tiles<KT>(a, q, tile * a.R, min((tile + 1) * a.R, q.n * a.G)).cost + a.item_cost;
 }
 
 // pre[s] = cost of the sequences before s over all heads, pre[n_seqs] = the total.  Every thread of the
@@ -194,20 +195,22 @@ struct AcRun {
 	uint32_t item;         // where the current item begins
 
 	__device__ __forceinline__ bool done() const { return at >= end; }
-	// this worker's key tiles of the item: [from, to)
-	__device__ __forceinline__ int from() const { return (int)(at - item); }
-	__device__ __forceinline__ int to() const { return (int)(min(end, item + (uint32_t)t.cost) - item); }
+	// this worker's key tiles of the item: [from, to), never none.  The item's own cost lies ahead of its tiles; a run
+	// that ends within it leaves the item to the next worker.
+	__device__ __forceinline__ int from() const { return max(0, (int)(at - item) - own_); }
+	__device__ __forceinline__ int to() const { return min((int)(end - item) - own_, t.cost); }
 	__device__ __forceinline__ bool whole() const { return from() == 0 && to() == t.cost; }
 	__device__ __forceinline__ int rows() const { return min(r_, rows_ - tile * r_); }
 	// slot of the partial: a worker ends at most one item that began before it and begins at most one
 	// that ends after it
 	__device__ __forceinline__ int slot(int worker) const { return 2 * worker + (from() == 0 ? 1 : 0); }
-	__device__ __forceinline__ int last_worker() const { return (int)((item + (uint32_t)t.cost - 1) / run); }
-	int r_, rows_; // rows of an item, rows of the sequence
+	__device__ __forceinline__ int last_worker() const { return (int)((item + (uint32_t)(own_ + t.cost) - 1) / run); }
+	int r_, rows_, own_; // rows of an item, rows of the sequence, the items' own cost
 
 	__device__ __forceinline__ void tile_of(const AttnChunkArgs& a)
 	{
 		t = ac_tiles<KT>(a, q, tile * r_, min((tile + 1) * r_, rows_));
+		if ((int)(end - item) <= own_) at = end;
 	}
 
 	// by a whole warp
@@ -220,6 +223,7 @@ struct AcRun {
 		at = b < total ? (uint32_t)b : total;
 		end = (uint32_t)min(b + run, (uint64_t)total);
 		r_ = a.R;
+		own_ = a.item_cost;
 		if (done()) return;
 		int l = 0, r = a.n_seqs; // the last s with pre[s] <= at
 		while (r - l > 1) {
@@ -270,7 +274,7 @@ struct AcRun {
 
 	__device__ __forceinline__ void next(const AttnChunkArgs& a, const uint32_t* pre)
 	{
-		item += (uint32_t)t.cost;
+		item += (uint32_t)(t.cost + own_);
 		at = item;
 		if (done()) return;
 		if (++tile == tiles) {

@@ -42,6 +42,9 @@ static_assert(2 * kCtRegsSoftmax + kCtRegsRest <= 3 * kCtRegsLaunch, "register s
 constexpr int kCtMaxStages = 12;
 constexpr uint32_t kCtAtom = 128 * 64 * 2; // one [128 x 64] bf16 SWIZZLE_128B block: 16 KB
 constexpr float kCtRescaleLog2 = 8.0f;  // growth of a row's max that O is not rescaled for
+// An item costs about 2 key tiles beside its own (its masked tiles, its last product's wait, its output): without
+// it the worker that met 16 items of a short prompt ended 30 us behind the others (8 chunks beside 24 decodes).
+constexpr int kCtItemCost = 2;
 constexpr uint32_t kCtBarBytes = 304;
 
 enum CtBar : int {
