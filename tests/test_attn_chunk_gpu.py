@@ -290,3 +290,10 @@ def test_pages_past_4_gb(cuda, H, KV, hd, dtype, spare):
     """Pools of 8.8 GB: half of the pages that a random draw takes lie beyond 32-bit byte offsets."""
     call = check(cuda, [(1, 300), (3, 40), (60, 200)], H, KV, hd, dtype, spare=spare, seed=6)
     assert int(call.c.table.max()) * KV * 16 * hd * call.c.k.element_size() > 1 << 32
+
+
+@pytest.mark.parametrize("KV,hd", [(8, 128), (3, 64)])
+def test_many_short_prompts_beside_a_long_one(cuda, KV, hd):
+    """Items of one to three key tiles, whose own cost is as large: cuts that fall before an item's first tile."""
+    check(cuda, [(69, 197)] * 10 + [(300, 1500)] + [(33, 40)] * 9 + [(1, 900), (130, 131)], 4 * KV, KV, hd, "bf16", seed=8)
+    check(cuda, [(20, 20)], 4 * KV, KV, hd, "bf16", seed=9)
