@@ -350,8 +350,9 @@ Error_t inf_qk_norm_rope(const InfPagedKv* kv, const InfQkNormRope* args, void* 
  *   window == 0  or  k > p - window  or  k < n_sink,
  * out = sum_k softmax_k(scale * q . K_k) V_k, softmax statistics and sums in fp32, fp32 accumulation.
  * bf16 caches with head_dim 64 or 128, a kv_block of 16, 32, 64 or 128 and at most 128 query heads
- * per KV head run on the tensor cores (the weights are rounded to bf16 for the second product);
- * others compute in fp32 throughout.
+ * per KV head run on the tensor cores: the weights are rounded to bf16 for the second product, for
+ * sequences of at most 16 rows per KV head (rows times the query heads of a KV head) to two bf16 parts
+ * (16 bits).  Others compute in fp32 throughout.
  * A row that sees nothing (p < 0) gets zeros; rows before q_start[0] and from q_start[n_seqs] on are
  * left as they were.  Pages that no row of a sequence sees may be missing (-1), and positions that no
  * row of it sees may hold anything, NaN included (a NaN that some row sees may reach the sequence's other

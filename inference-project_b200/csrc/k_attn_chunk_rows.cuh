@@ -8,9 +8,10 @@
 // the 16 rows of the A tile, S = Q.K^T with K fragments from ldmatrix, the accumulator fragments of S are the
 // A fragments of P.V, V comes from ldmatrix.trans.  A warp whose run ends inside an item stores its share, which
 // k_attn_chunk_combine joins with the others.
-// Rounding: S, O, max and sum in fp32; P is rounded to bf16 for the second product, the sum adds the unrounded
-// weights.  V positions that no row of the item sees are masked out of the fragments (only where such a tile
-// exists: its ends).
+// Rounding: S, O, max and sum in fp32; P goes into the second product as two bf16 parts (rounded, then the
+// rounding of what that left over: 16 bits, so that a row's error is its output's rounding), the sum adds the
+// unrounded weights.  V positions that no row of the item sees are masked out of the fragments (only where such
+// a tile exists: its ends).
 #pragma once
 
 #include "k_attn_chunk.cuh"
@@ -190,8 +191,13 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 			for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
 				for (int j = 0; j < 4; ++j) p[nt][j] = ex2_approx(fmaf(s[nt][j], sl2, -mu[j >> 1]));
-			const uint32_t pa[4] = {pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]),
-			                        pack_bf16(p[1][2], p[1][3])};
+			uint32_t pa[4], pr[4]; // P = pa + pr: rounded, and what is left rounded again
+#pragma unroll
+			for (int f = 0; f < 4; ++f) {
+				const float x = p[f >> 1][(f & 1) * 2], y = p[f >> 1][(f & 1) * 2 + 1];
+				pa[f] = pack_bf16(x, y);
+				pr[f] = pack_bf16(x - __uint_as_float(pa[f] << 16), y - __uint_as_float(pa[f] & 0xFFFF0000u));
+			}
 #pragma unroll
 			for (int e = 0; e < 2; ++e)
 				l[e] = fmaf(l[e], al[e], (p[0][2 * e] + p[0][2 * e + 1]) + (p[1][2 * e] + p[1][2 * e + 1]));
@@ -216,8 +222,11 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 			for (int dt = 0; dt < HD / 8; dt += 2) {
 				uint32_t b0, b1, c0, c1;
 				ldsm_x4_trans(vc + cr_off<HD>((mi & 1) * 8 + mr, dt + (mi >> 1)), b0, b1, c0, c1);
-				mma_bf16_16816(o[dt], pa, b0 & keep0, b1 & keep1);
-				mma_bf16_16816(o[dt + 1], pa, c0 & keep0, c1 & keep1);
+				b0 &= keep0, b1 &= keep1, c0 &= keep0, c1 &= keep1;
+				mma_bf16_16816(o[dt], pr, b0, b1);
+				mma_bf16_16816(o[dt + 1], pr, c0, c1);
+				mma_bf16_16816(o[dt], pa, b0, b1);
+				mma_bf16_16816(o[dt + 1], pa, c0, c1);
 			}
 			__syncwarp(); // every lane is done with the stage
 			fetch();
