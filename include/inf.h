@@ -390,8 +390,9 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 Error_t inf_kv_copy_pages(const InfPagedKv* kv, const i32* d_src, const i32* d_dst, u32 n, i32* d_status, void* stream);
 /* Entries d_first[i] .. d_last[i] - 1 of slot d_slot[i] are given up: each page they name loses one
  * reference and the entry becomes -1 (d_first NULL: 0; d_last NULL: pages_per_seq).  An entry named
- * twice is given up once.  Frees whole sequences, or the pages that left a sliding window.  A slot or
- * range outside the table is reported (ErrorInvalidValue) and skipped, an entry outside the pool or a
+ * twice is given up once.  Frees whole sequences, or the pages that left a sliding window.  A range of
+ * the table whose first is not below its last is empty.  A slot outside the table, a first or a last
+ * outside 0 .. pages_per_seq is reported (ErrorInvalidValue) and skipped, an entry outside the pool or a
  * page without references too (the entry becomes -1). */
 Error_t inf_kv_free(const InfPagedKv* kv, const i32* d_slot, const i32* d_first, const i32* d_last, u32 n, i32* d_status,
                     void* stream);

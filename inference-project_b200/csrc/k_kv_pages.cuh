@@ -130,7 +130,8 @@ __global__ void __launch_bounds__(kPgThreads) k_kv_free(const PageFreeArgs a, ui
 	pdl_trigger();
 	for (uint32_t i = blockIdx.y; i < n; i += gridDim.y) {
 		const int slot = a.slot[i], first = a.first ? a.first[i] : 0, last = a.last ? a.last[i] : a.pages_per_seq;
-		if (slot < 0 || slot >= a.n_slots || first < 0 || last > a.pages_per_seq) {
+		// both ends within the table: entry indices fit 31 bits with a grid's width to spare (pages_per_seq <= 2^30)
+		if (slot < 0 || slot >= a.n_slots || first < 0 || first > a.pages_per_seq || last < 0 || last > a.pages_per_seq) {
 			if (blockIdx.x == 0 && threadIdx.x == 0) report_err(a.status, kDevBadIndex);
 			continue;
 		}
