@@ -55,13 +55,16 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 	(void)sm_count(&sms);
 	P->n_pass = 0;
 	P->scratch = 0;
-	auto add = [&](ChunkPass p, u64 units) -> Error_t {
+	// The scratch is laid out for `most` workers, which do not depend on n_seqs: a call of fewer sequences, whose
+	// smaller prefix lets more workers onto an SM, fits where a call of more did.
+	auto add = [&](ChunkPass p, u64 units, int most) -> Error_t {
 		if (units > 0x7FFFFFFFull) return fail(ErrorUnsupported, "%s: %u tokens of %u positions at most", who, n_tokens, kv->pages_per_seq * kv->kv_block);
-		p.workers = (int)std::max<u64>(1, std::min<u64>(p.workers, (units + p.min_run - 1) / p.min_run));
+		const u64 runs = std::max<u64>(1, (units + p.min_run - 1) / p.min_run), room = std::min<u64>(most, runs);
+		p.workers = (int)std::min<u64>(p.workers, runs);
 		p.part_off = P->scratch;
-		P->scratch += up256((u64)2 * p.workers * ac_part_floats(p.R, (int)kv->head_dim) * sizeof(float));
+		P->scratch += up256(2 * room * ac_part_floats(p.R, (int)kv->head_dim) * sizeof(float));
 		p.jobs_off = P->scratch;
-		P->scratch += up256((u64)p.workers * kAcJobInts * sizeof(int));
+		P->scratch += up256(room * kAcJobInts * sizeof(int));
 		P->pass[P->n_pass++] = p;
 		return Success;
 	};
@@ -80,7 +83,7 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 			r.min_run = 4;
 			r.smem = attn_chunk_rows_smem((int)kv->head_dim, (int)n_seqs);
 			r.workers = sms * kCrWarps;
-			INF_TRY(add(r, (u64)std::min(n_seqs, n_tokens) * kv->n_kv_heads * (((u64)kv->pages_per_seq * blk + kCrKT - 1) / kCrKT + 1)));
+			INF_TRY(add(r, (u64)std::min(n_seqs, n_tokens) * kv->n_kv_heads * (((u64)kv->pages_per_seq * blk + kCrKT - 1) / kCrKT + 1), r.workers));
 		}
 		ChunkPass t = {};
 		t.kind = ChunkPass::TC;
@@ -91,7 +94,7 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 		t.min_run = 2 + kCtItemCost;
 		t.smem = ct_layout((int)kv->head_dim, (int)n_seqs).total;
 		t.workers = sms;
-		return add(t, units_max(kv, n_heads, n_tokens, n_seqs, (u32)t.R, kCtKT, kCtItemCost));
+		return add(t, units_max(kv, n_heads, n_tokens, n_seqs, (u32)t.R, kCtKT, kCtItemCost), t.workers);
 	}
 	ChunkPass f = {};
 	f.kind = ChunkPass::F32;
@@ -99,8 +102,9 @@ Error_t chunk_plan(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs, 
 	f.R = kAfR;
 	f.min_run = 2;
 	f.smem = attn_chunk_f32_smem((int)kv->head_dim, (int)n_seqs);
-	f.workers = sms * (int)std::max<u64>(1, std::min<u64>(8, (200u << 10) / f.smem));
-	return add(f, units_max(kv, n_heads, n_tokens, n_seqs, kAfR, kAfKT, 0));
+	auto ctas = [&](size_t smem) { return sms * (int)std::max<u64>(1, std::min<u64>(8, (200u << 10) / smem)); };
+	f.workers = ctas(f.smem);
+	return add(f, units_max(kv, n_heads, n_tokens, n_seqs, kAfR, kAfKT, 0), ctas(attn_chunk_f32_smem((int)kv->head_dim, 0)));
 }
 
 template <typename T>
