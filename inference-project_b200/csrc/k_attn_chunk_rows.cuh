@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 			                                                        (uint64_t)(run.q.row0 + tok) * a.q_stride + (uint64_t)head * HD);
 #pragma unroll
 			for (int ks = 0; ks < HD / 16; ++ks) {
-				qa[ks][e] = valid ? __ldg(src + ks * 8 + (gc >> 1)) : 0u;
-				qa[ks][2 + e] = valid ? __ldg(src + ks * 8 + (gc >> 1) + 4) : 0u;
+				qa[ks][e] = valid ? src[ks * 8 + (gc >> 1)] : 0u;
+				qa[ks][2 + e] = valid ? src[ks * 8 + (gc >> 1) + 4] : 0u;
 			}
 		}
 		const int first_pos = base_pos, last_pos = base_pos + a.group.div(rows - 1);
