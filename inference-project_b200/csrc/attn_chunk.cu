@@ -233,17 +233,13 @@ Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* str
 		on[0] = !on[1] || (u64)a.n_seqs * (u64)a.max_new < (u64)a.n_tokens || (slack + kCrRows / a.G) >= (u64)a.max_new;
 		if (!on[0]) P.pass[1].rows_min = 0;
 	}
-	int before = 0; // passes of this call that are running
 	for (int i = 0; i < P.n_pass; ++i) {
 		if (!on[i]) continue;
 		const ChunkPass& p = P.pass[i];
-		AttnChunkArgs b = pass_args(p);
-		// the second pass needs nothing of the first: it starts as soon as SMs are free, and waits at its end
-		b.late_wait = before > 0;
+		const AttnChunkArgs b = pass_args(p);
 		if (p.kind == ChunkPass::Rows) INF_TRY(a.hd == 64 ? launch_rows<64>(b, p, st) : launch_rows<128>(b, p, st));
 		else if (p.kind == ChunkPass::TC) INF_TRY(a.hd == 64 ? launch_tc<64>(b, p, st) : launch_tc<128>(b, p, st));
 		else INF_TRY(kv->dtype == InfBF16 ? launch_f32<bf16>(b, p, st) : launch_f32<float>(b, p, st));
-		++before;
 	}
 	for (int i = 0; i < P.n_pass; ++i) {
 		if (!on[i]) continue;

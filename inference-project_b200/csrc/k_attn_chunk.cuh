@@ -60,7 +60,6 @@ struct AttnChunkArgs {
 	int workers;
 	int min_run;                   // cost of a worker's run at least
 	int item_cost;                 // what an item costs beside its key tiles, in key tiles
-	int late_wait;                 // this kernel may run beside the one before it and waits for it at its end
 	float* part;                   // [2 * workers][hd + 2][R] partial O (unnormalised), max (log2 units), sum
 	int* jobs;                     // [workers][kAcJobInts]: the item that a worker begins and others end
 };

@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 		asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
 		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 	}
-	if (!a.late_wait) pdl_wait();
+	pdl_wait();
 	pdl_trigger();
 	tc_fence_before();
 	ac_prefix<kCtKT>(a, pre); // ends with a barrier
@@ -594,8 +594,6 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 		tc_fence_after();
 		asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 	}
-	// what comes after this kernel may count on the one before it, too
-	if (a.late_wait) pdl_wait();
 }
 
 } // namespace inf

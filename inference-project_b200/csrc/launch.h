@@ -1,5 +1,7 @@
-// Launching the stand-alone kernels of the paged-cache operators: every one starts with
-// griddepcontrol.wait, so it may be launched while the kernel before it on the stream drains.
+// Launching the stand-alone kernels of the paged-cache operators: every one waits (griddepcontrol.wait) before
+// it touches memory, so it may be launched while the kernel before it on the stream drains, and lets the
+// next one start only behind that wait.  Memory is visible to the grid that waits and no other: a kernel that
+// counted on the wait of the one before it would read without a promise, though that one had completed.
 #pragma once
 
 #include <mutex>
