@@ -359,7 +359,9 @@ Error_t inf_qk_norm_rope(const InfPagedKv* kv, const InfQkNormRope* args, void* 
  * rows).  Query heads h use KV head h / (n_heads / n_kv_heads).
  * Rows outside q, more than max_new rows, a slot or context outside the tables: reported
  * (ErrorInvalidValue / ErrorKvOutOfRange), the sequence skipped; a page outside the pool that a row
- * sees: reported, the sequence's outputs unspecified.  n_seqs at most 4096. */
+ * sees: reported, the sequence's outputs unspecified.  n_seqs at most 4096.  q_start, ctx_len, seq_slot
+ * and the tables may not change while the call's kernels run: its outputs and its scratch are then
+ * unspecified, and it may end with ErrorTimeout. */
 typedef struct InfAttnChunk {
 	const void* q;         /* [n_tokens] rows of n_heads * head_dim, 16-byte aligned */
 	void*       out;       /* [n_tokens] rows of n_heads * head_dim, 16-byte aligned, not q */

@@ -183,7 +183,9 @@ __device__ __forceinline__ void ac_prefix(const AttnChunkArgs& a, uint32_t* pre)
 	__syncthreads();
 }
 
-// A worker's run of the laid-out costs, walked item by item (every lane of the warp holds the same).
+// A worker's run of the laid-out costs, walked item by item (every lane of the warp holds the same).  Lengths are
+// read again at every sequence; where they are no longer those of the prefix (a caller that changed them under
+// the kernel) the run ends, or goes on over positions inside the tables.
 // kOneTile: sequences of at most R rows only.
 template <int KT, bool kOneTile = false>
 struct AcRun {
@@ -212,6 +214,14 @@ struct AcRun {
 		if ((int)(end - item) <= own_) at = end;
 	}
 
+	__device__ __forceinline__ void sequence(const AttnChunkArgs& a)
+	{
+		q = ac_seq(a, s, false);
+		rows_ = q.n * a.G;
+		tiles = (rows_ + r_ - 1) / r_;
+		if (rows_ == 0) at = end; // lengths that changed
+	}
+
 	// by a whole warp
 	__device__ __forceinline__ void begin(const AttnChunkArgs& a, const uint32_t* pre, int worker)
 	{
@@ -231,9 +241,8 @@ struct AcRun {
 			else r = m;
 		}
 		s = l;
-		q = ac_seq(a, s, false);
-		rows_ = q.n * a.G;
-		tiles = (rows_ + r_ - 1) / r_;
+		sequence(a);
+		if (done()) return;
 		const uint32_t per_head = (pre[s + 1] - pre[s]) / (uint32_t)a.KV;
 		const uint32_t in = at - pre[s];
 		h = (int)(in / per_head);
@@ -242,6 +251,7 @@ struct AcRun {
 		if (kOneTile) {
 			tile = 0;
 			tile_of(a);
+			if (from() >= t.cost) at = end; // lengths that changed
 			return;
 		}
 		// the tile that holds `left`: 32 tiles at a time
@@ -268,7 +278,7 @@ struct AcRun {
 			}
 		}
 		if (found) tile_of(a);
-		else end = at; // lengths that changed under the kernel: the run ends
+		else at = end; // lengths that changed
 	}
 
 	__device__ __forceinline__ void next(const AttnChunkArgs& a, const uint32_t* pre)
@@ -282,13 +292,12 @@ struct AcRun {
 				h = 0;
 				do ++s;
 				while (s < a.n_seqs && pre[s + 1] == pre[s]);
-				if (s >= a.n_seqs) { // as above
-					end = at;
+				if (s >= a.n_seqs) { // lengths that changed
+					at = end;
 					return;
 				}
-				q = ac_seq(a, s, false);
-				rows_ = q.n * a.G;
-				tiles = (rows_ + r_ - 1) / r_;
+				sequence(a);
+				if (done()) return;
 			}
 		}
 		tile_of(a);
@@ -305,7 +314,7 @@ __device__ __forceinline__ void ac_job(const AttnChunkArgs& a, int w, const Run&
 	j[kAcJobHead] = run.h;
 	j[kAcJobRow] = run.tile * a.R;
 	j[kAcJobRows] = run.rows();
-	j[kAcJobLast] = run.last_worker();
+	j[kAcJobLast] = min(run.last_worker(), a.workers - 1); // (lengths that changed)
 }
 
 // floats of one partial: R rows of O, each row's max and sum

@@ -265,8 +265,9 @@ __global__ void __launch_bounds__(kCrThreads, 1)
 		}
 		if (!whole && run.from() == 0 && lane == 0) ac_job(a, worker, run);
 	}
-	if (!ok && lane == 0) {
-		// never leave the CTA with copies in flight
+	if (lane == 0) {
+		// never leave the CTA with copies in flight: there are some behind a wait that ran out, or where lengths
+		// changed between a copy and its products
 		for (int i = max(0, issued - kStages); i < issued; ++i) {
 			const long long t0 = clock64();
 			while (!mbar_try_wait(&bars[i % kStages], (uint32_t)(i / kStages) & 1u))

@@ -269,17 +269,14 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 					r.skip(2, stages);
 				}
 			}
-			if (!ok) {
-				// never leave the CTA with copies in flight: this producer's last entries
-				__syncwarp();
-				CtRing back;
-				if (is_v) back.next(stages);
-				for (uint32_t i = is_v ? 1u : 0u; i < entry; i += 2, back.skip(2, stages)) {
-					if (i + (uint32_t)stages < entry) continue;
-					const uint64_t t0 = global_timer_ns();
-					while (!mbar_try_wait(&bars[kCtFull + back.stage], back.phase))
-						if (global_timer_ns() - t0 > kWaitLimitNs) break;
-				}
+			// never leave the CTA with copies in flight (there are some behind a wait that ran out, or where lengths
+			// changed between a copy and its products): this producer's last entries
+			__syncwarp();
+			for (uint32_t back = 2; back <= (uint32_t)stages && back <= entry; back += 2) {
+				const uint32_t i = entry - back, use = i / (uint32_t)stages;
+				const uint64_t t0 = global_timer_ns();
+				while (!mbar_try_wait(&bars[kCtFull + (i - use * (uint32_t)stages)], use & 1u))
+					if (global_timer_ns() - t0 > kWaitLimitNs) break;
 			}
 		} else if (warp == 9) {
 			// ---------------- product issuer: the warp runs the pipeline converged, one elected lane issues
@@ -410,13 +407,11 @@ __global__ void __launch_bounds__(kCtThreads, 1)
 					++uses[sub];
 				}
 			}
-			if (!ok) {
-				for (int sub = 0; sub < 2; ++sub) { // copies in flight
-					if (uses[sub] == 0) continue;
-					const long long t0 = clock64();
-					while (!mbar_try_wait(&bars[kCtQ + sub], (uses[sub] - 1) & 1u))
-						if (clock64() - t0 > kWaitLimitCycles) break;
-				}
+			for (int sub = 0; sub < 2; ++sub) { // copies in flight
+				if (uses[sub] == 0) continue;
+				const long long t0 = clock64();
+				while (!mbar_try_wait(&bars[kCtQ + sub], (uses[sub] - 1) & 1u))
+					if (clock64() - t0 > kWaitLimitCycles) break;
 			}
 		}
 	} else {
