@@ -306,7 +306,7 @@ typedef struct InfPagedKv {
 	u32   dtype;        /* InfDtype */
 } InfPagedKv;
 /* Waits for `stream`, reads the status word, clears it and returns the failure it held (Success if
- * none).  Not for a capturing stream. */
+ * none).  ErrorInvalidValue on a capturing stream; the capture goes on. */
 Error_t inf_check_status(i32* d_status, void* stream);
 
 /* The projected rows of new tokens into the cache, one pass: per token and head, with x the head's

@@ -115,6 +115,10 @@ extern "C" {
 Error_t inf_check_status(i32* d_status, void* stream)
 {
 	INF_TRY(check_dev_arg("inf_check_status", "status", d_status, 4));
+	// a wait would invalidate the capture
+	cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+	INF_CUDA_TRY(cudaStreamIsCapturing((cudaStream_t)stream, &capture));
+	if (capture != cudaStreamCaptureStatusNone) return fail(ErrorInvalidValue, "inf_check_status: the stream is capturing");
 	i32 v = 0;
 	INF_CUDA_TRY(cudaMemcpyAsync(&v, d_status, sizeof v, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
 	INF_CUDA_TRY(cudaMemsetAsync(d_status, 0, sizeof v, (cudaStream_t)stream));
