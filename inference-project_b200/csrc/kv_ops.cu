@@ -80,6 +80,16 @@ PagePools page_pools(const InfPagedKv* kv)
 	return P;
 }
 
+// The kernels count a page's pieces (slices of K and V, or heads, over all layers) in 32 bits.
+Error_t check_page_pieces(const char* who, const InfPagedKv* kv)
+{
+	const PagePools P = page_pools(kv);
+	const u64 slices = ((u64)P.page_bytes + kPgSlice - 1) / kPgSlice;
+	if (2 * (u64)kv->n_layers * std::max<u64>(slices, kv->n_kv_heads) > 0x7FFFFFFFull)
+		return fail(ErrorUnsupported, "%s: %u layers of %u bytes a page", who, kv->n_layers, P.page_bytes);
+	return Success;
+}
+
 // CTAs of a copy of `bytes`: a warp per slice up to eight CTAs on every SM.
 unsigned copy_ctas(u64 bytes, int sms)
 {
@@ -193,6 +203,7 @@ Error_t inf_kv_copy_pages(const InfPagedKv* kv, const i32* d_src, const i32* d_d
 {
 	const char* who = "inf_kv_copy_pages";
 	INF_TRY(check_paged_kv(who, kv, 0, false));
+	INF_TRY(check_page_pieces(who, kv));
 	if (n > kv->n_pages) return fail(ErrorInvalidValue, "%s: %u pairs in %u pages", who, n, kv->n_pages);
 	if (n == 0) return Success;
 	INF_TRY(check_paged_kv_pointers(who, kv, false, false));
@@ -237,6 +248,7 @@ Error_t inf_kv_fork(const InfPagedKv* kv, const i32* d_src, const i32* d_dst, co
 {
 	const char* who = "inf_kv_fork";
 	INF_TRY(check_paged_kv(who, kv, 0, true));
+	INF_TRY(check_page_pieces(who, kv));
 	if (n > kv->n_slots) return fail(ErrorInvalidValue, "%s: %u forks into %u slots", who, n, kv->n_slots);
 	if (n == 0) return Success;
 	if (scratch_bytes < inf_kv_pages_scratch_bytes(kv)) return fail(ErrorInvalidValue, "%s: scratch too small", who);
@@ -275,6 +287,7 @@ Error_t inf_kv_compact(const InfPagedKv* kv, i32* d_map, i32* d_n_live, void* d_
 {
 	const char* who = "inf_kv_compact";
 	INF_TRY(check_paged_kv(who, kv, 0, true));
+	INF_TRY(check_page_pieces(who, kv));
 	if (kv->n_pages > kCompactMaxPages) return fail(ErrorUnsupported, "%s: %u pages, above %u", who, kv->n_pages, kCompactMaxPages);
 	if (scratch_bytes < inf_kv_pages_scratch_bytes(kv)) return fail(ErrorInvalidValue, "%s: scratch too small", who);
 	INF_TRY(check_paged_kv_pointers(who, kv, true, true));
