@@ -104,7 +104,10 @@ __global__ void __launch_bounds__(kPgThreads) k_kv_copy_pages(const PageCopyArgs
 		dst = a.dst[i];
 		bool ok = src >= 0 && src < a.P.n_pages && dst >= 0 && dst < a.P.n_pages;
 		// a page written twice, or read by another pair while it is written, has no order to go by.
-		// The scan is 4 n bytes of L2 per pair and warp, against megabytes copied per pair.
+		// The scan reads both lists, 8 n bytes from L2, for every pair that a warp enters: nothing beside the copy of
+		// pages of many layers (22 layers of 4 x 16 x 64 bf16: 5.4 TB/s at 4000 pairs, 4.5 at 16000), but more than
+		// the copy where one layer's small pages go by the thousand (4000 pairs of 16 KB, K and V: 124 us, 20 at the
+		// copy rate; of 64 KB: 169 us, 80).
 		for (uint32_t j = lane; j < a.n; j += kWarp) ok = ok && !(j < i && a.dst[j] == dst) && a.src[j] != dst;
 		ok = __all_sync(0xFFFFFFFFu, ok);
 		if (!ok && lane == 0) report_err(a.status, kDevBadIndex);
@@ -203,7 +206,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_fork_plan(const ForkArgs a)
 	pdl_wait();
 	pdl_trigger();
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	// one warp per fork: its numbers, the other forks' slots, its destination row
+	// one warp per fork: its numbers, the other forks' slots (n^2 / 32 steps in all, in one CTA: 30 us a call at 256
+	// forks, 146 at 1024, 1.7 ms at 4096), its destination row
 	for (uint32_t i = warp; i < a.n; i += kPlanThreads / kWarp) {
 		const int s = a.src[i], d = a.dst[i], len = a.len[i];
 		bool ok = s >= 0 && s < a.n_slots && d >= 0 && d < a.n_slots && len >= 0 && len <= a.pages_per_seq * a.kv_block;
