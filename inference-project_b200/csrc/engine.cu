@@ -200,13 +200,13 @@ static Error_t tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000* out)
 	return Success;
 }
 
-Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages, u32 box_rows)
+Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages)
 {
 	PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
 	INF_TRY(tensor_map_encoder(&encode));
 	const cuuint64_t dims[4] = {hd, blk, kv, pages};
 	const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)blk * hd * 2, (cuuint64_t)kv * blk * hd * 2};
-	const cuuint32_t box[4] = {64, box_rows ? box_rows : blk, 1, box_pages};
+	const cuuint32_t box[4] = {64, blk, 1, box_pages};
 	const cuuint32_t estr[4] = {1, 1, 1, 1};
 	const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
 	                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

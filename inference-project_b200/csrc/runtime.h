@@ -36,8 +36,8 @@ bool is_local_device_ptr(const void* p);
 Error_t map_dev_err(int v);
 
 // A layer's paged K or V pool [pages][KV][blk][hd] as a 4-D tensor (hd, row, head, page) with boxes
-// of 64 head dims x box_rows rows (0: blk) x 1 head x box_pages pages, SWIZZLE_128B.
-Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages, u32 box_rows = 0);
+// of 64 head dims x blk rows x 1 head x box_pages pages, SWIZZLE_128B.
+Error_t tensor_map_kv(CUtensorMap* m, const void* base, u32 hd, u32 blk, u32 kv, u32 pages, u32 box_pages);
 // Rows of `heads` heads of hd, `stride` elements apart, as a 3-D tensor (dim, head, token) with boxes of 64 dims x
 // box_heads x box_tokens, SWIZZLE_128B.
 Error_t tensor_map_q(CUtensorMap* m, const void* base, u32 tokens, u32 heads, u32 hd, u64 stride, u32 box_heads, u32 box_tokens);
