@@ -382,7 +382,7 @@ typedef struct InfAttnChunk {
 	u32         n_sink;
 	u32         layer;
 } InfAttnChunk;
-/* Enough for every call of at most as many tokens and sequences; 0: not a shape that inf_attn_chunk takes. */
+/* Enough for every call of at most as many tokens and sequences; 0 where heads or counts are refused. */
 u64     inf_attn_chunk_scratch_bytes(const InfPagedKv* kv, u32 n_heads, u32 n_tokens, u32 n_seqs);
 Error_t inf_attn_chunk(const InfPagedKv* kv, const InfAttnChunk* args, void* stream);
 

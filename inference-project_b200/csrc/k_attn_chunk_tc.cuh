@@ -18,8 +18,10 @@
 // warpgroup issued its own products both waited and both computed at the same time), and makes a completed
 // S(j+1) imply a completed PV(j): O may then be rescaled without another wait.  That happens only when a
 // row's max grows by more than 2^8 (bf16 and fp32 hold the larger weights as well, and O / sum is unchanged).
-// Rounding: S, O, max and sum are fp32; P is rounded to bf16 for the second product, the sum adds the
-// unrounded weights (their rounding errors are independent and average out).
+// Rounding: S, O, max and sum are fp32; P is rounded to bf16 for the second product, as in the library's prefill
+// attention, the sum adds the unrounded weights.  The weights' roundings are independent of each other and add
+// about as much to a row's error as the output's own (root mean square 0.0023 of the outputs, 0.0017 with exact
+// weights); a second bf16 part, which the row kernel has, would double P.V on the tensor pipe here.
 // Positions that no row of the item sees are not loaded page by page; where they share a page with seen
 // ones, their V rows are overwritten by zeros in shared memory before the product, so that nothing they
 // hold (NaN included) reaches a sum; their scores are dropped by the mask.
